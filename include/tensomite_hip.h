@@ -401,6 +401,75 @@ int tmh_add(uint64_t a, uint64_t b, uint64_t dst, uint64_t count);
  * of the highest value of row r (rows `ldx` apart). */
 int tmh_argmax(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t ids);
 
+/* -------------------------------------- a cache in pages, and sampling (serving)
+ *
+ * What a server of many sequences runs beside the ops above; the reference
+ * has no counterpart (its caches are rows of fixed capacity and its server
+ * samples on the host), so these promise F32 accuracy, not a host's bits.
+ * The cache is `pages` pages of `page_size` positions, keys and values each
+ * [pages, kv_heads, page_size, width], shared by `sequences` sequences whose
+ * metadata is in device memory:
+ *
+ *   page_table  int32 [sequences, table_width]: sequence s holds position p on
+ *               page page_table[s][p / page_size], at place p % page_size;
+ *               entries past a sequence's last position are not read
+ *   starts      int32 [sequences + 1]: rows starts[s] ... starts[s+1] - 1 of the
+ *               call's tokens are sequence s's new tokens, its newest
+ *               positions; rows of no sequence are left as they were
+ *   lengths     int32 [sequences]: positions s holds, the new ones among them
+ *
+ * so row starts[s] + i is at position lengths[s] - (starts[s+1] - starts[s]) + i.
+ * A sequence whose numbers do not fit (rows past `tokens`, falling starts, a
+ * length below its new tokens or past the table) is skipped, its rows left as
+ * they were; a page out of range is not read or written, and the rows that
+ * see it are unspecified. Both are index errors, reported at tmh_sync.
+ * `kind` is the cache's element type (ggml's numbering, as tmh_gguf_tensor's);
+ * keys and values are 16-byte aligned, width a multiple of 8 up to 256, and
+ * pages * kv_heads * page_size below 2^31. */
+#define TMH_CACHE_F32 0
+#define TMH_CACHE_F16 1
+#define TMH_CACHE_BF16 30
+
+/* RoPE of the q and k heads and the cache write of the rotated k and the v
+ * heads, as tmh_rope_write (the same bits in q_dst and an F32 cache; F16 and
+ * BF16 elements are the nearest, ties to even), into pages. x rows are `ldx`
+ * apart; a position's rotation is its row of the cos/sin tables ([table_rows,
+ * width]); a position past them is an index error. */
+int tmh_rope_write_paged(uint64_t x, uint32_t ldx, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                         uint64_t cos, uint64_t sin, uint32_t table_rows, uint32_t kind, uint32_t pages,
+                         uint32_t page_size, uint64_t page_table, uint32_t table_width, uint32_t sequences,
+                         uint64_t starts, uint64_t lengths, uint64_t q_dst, uint64_t keys, uint64_t values);
+
+/* Attention of each sequence's new tokens over its pages: for the token at
+ * position p and each head, softmax over the visible positions j of
+ * scale * q.k_j, times v_j. Visible: j <= p and, with a window, j > p - window
+ * or j < sinks (the first `sinks` positions stay visible); window 0 is no
+ * window. What hidden positions hold, NaN and infinity included, does not
+ * reach a result. Query head h reads kv head h / (heads / kv_heads); q rows
+ * are `ldq` apart ([heads, width] each), dst rows `ld_dst` apart, both F32.
+ * No sequence may have more than `max_new` new tokens or `max_length`
+ * positions (they size the launch). */
+int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t heads, uint32_t kind, uint64_t keys,
+                        uint64_t values, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t width,
+                        uint64_t page_table, uint32_t table_width, uint32_t sequences, uint64_t starts,
+                        uint64_t lengths, uint32_t max_new, uint32_t max_length, uint32_t window, uint32_t sinks,
+                        float scale, uint64_t dst, uint32_t ld_dst);
+
+/* The next token of each row of logits (rows `ldx` apart) from the row's own
+ * settings, arrays [rows] in device memory: ids[r] (int32). Candidates stand
+ * by falling logit, equal ones by rising index, with weight
+ * e^((x - highest) / temperature[r]). The first top_k[r] (int32; below 1: all)
+ * stay; of those the shortest run from the front whose weights reach top_p[r]
+ * of their sum (1 or more: all); of those the ones of weight at least
+ * min_p[r] of the highest; the first always stays. Chosen is the first whose running sum
+ * passes u[r] (f32 in [0, 1)) times the sum of what stayed. temperature[r]
+ * not above 0 is tmh_argmax. temperature, top_k, top_p and min_p may each be 0
+ * (no array): 1, all, 1 and 0. Sums and the weights are in 64 bits: the same
+ * inputs give the same ids on every call. NaN is never chosen while another
+ * candidate is there; n is at most 2^24. */
+int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t temperature, uint64_t top_k,
+               uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids);
+
 /* ------------------------------------------------------------ Llama decoding
  *
  * A Llama whose forward runs entirely on the device: Llama#forward /

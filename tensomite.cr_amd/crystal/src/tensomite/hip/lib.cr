@@ -29,6 +29,10 @@ module Tensomite
     Q4_0 = 1_u32
     Q4_1 = 2_u32
 
+    CACHE_F32  =  0_u32
+    CACHE_F16  =  1_u32
+    CACHE_BF16 = 30_u32
+
     X_F32       = 0_u32
     X_RMSNORM   = 1_u32
     X_QUANTISED = 2_u32
@@ -182,6 +186,24 @@ module Tensomite
                             dst : DevicePtr) : Int32
     fun add = tmh_add(a : DevicePtr, b : DevicePtr, dst : DevicePtr, count : UInt64) : Int32
     fun argmax = tmh_argmax(x : DevicePtr, ldx : UInt32, rows : UInt32, n : UInt32, ids : DevicePtr) : Int32
+
+    # a cache in pages, and sampling
+    fun rope_write_paged = tmh_rope_write_paged(x : DevicePtr, ldx : UInt32, tokens : UInt32, heads : UInt32,
+                                                kv_heads : UInt32, width : UInt32, cos : DevicePtr, sin : DevicePtr,
+                                                table_rows : UInt32, kind : UInt32, pages : UInt32,
+                                                page_size : UInt32, page_table : DevicePtr, table_width : UInt32,
+                                                sequences : UInt32, starts : DevicePtr, lengths : DevicePtr,
+                                                q_dst : DevicePtr, keys : DevicePtr, values : DevicePtr) : Int32
+    fun attention_paged = tmh_attention_paged(q : DevicePtr, ldq : UInt32, tokens : UInt32, heads : UInt32,
+                                              kind : UInt32, keys : DevicePtr, values : DevicePtr, pages : UInt32,
+                                              page_size : UInt32, kv_heads : UInt32, width : UInt32,
+                                              page_table : DevicePtr, table_width : UInt32, sequences : UInt32,
+                                              starts : DevicePtr, lengths : DevicePtr, max_new : UInt32,
+                                              max_length : UInt32, window : UInt32, sinks : UInt32, scale : Float32,
+                                              dst : DevicePtr, ld_dst : UInt32) : Int32
+    fun sample = tmh_sample(x : DevicePtr, ldx : UInt32, rows : UInt32, n : UInt32, temperature : DevicePtr,
+                            top_k : DevicePtr, top_p : DevicePtr, min_p : DevicePtr, u : DevicePtr,
+                            ids : DevicePtr) : Int32
 
     # the device-resident Llama decoder
     fun llama_create = tmh_llama_create(config : LlamaConfig*, weights : LlamaWeights*, rows : UInt32,

@@ -345,6 +345,21 @@ int device_context(DeviceContext* out, bool kernels);
 void note_launch(int index, int ops, bool errors);
 // Device allocation honouring the allocation-failure test hook.
 hipError_t device_malloc(void** p, size_t bytes);
+// Device memory of at least `bytes` for the launches of one call, one array a
+// device, kept and grown: held by the call until its last launch is queued, so
+// that two threads' launches do not take turns in it.
+class Workspace {
+public:
+    Workspace(int index, size_t bytes);
+    ~Workspace();
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    int status;       // a TMH_* code
+    uint8_t* memory;  // 256-byte aligned
+
+private:
+    int index;
+};
 // Bytes the quantise pass writes for `rows` rows of k, and its carving.
 size_t scratch_need(uint32_t rows, uint32_t k);
 Activations carve_scratch(uint8_t* base, uint32_t rows, uint32_t k);

@@ -124,6 +124,12 @@ struct Device {
     uint8_t* act_scratch = nullptr;
     size_t act_scratch_bytes = 0;
 
+    // Scratch of the operators that split a row's work over workgroups and
+    // join it in a second launch, grown as act_scratch is.
+    std::mutex work;
+    uint8_t* work_scratch = nullptr;
+    size_t work_scratch_bytes = 0;
+
     // This device's copy of the file-scope `scratch` array, looked up once at
     // set-up (the allocation-free entry point's quantised activations), and
     // the lock that keeps its quantise pass and product adjacent on the stream.
@@ -218,23 +224,25 @@ void recycle_retired(Device& d) {
     });
 }
 
-// Grows the activation scratch to at least `bytes`, waiting for the work
-// that may still read the old one.
-int ensure_scratch(Device& d, size_t bytes) {
-    if (bytes <= d.act_scratch_bytes) return TMH_SUCCESS;
+// Grows a scratch array to at least `bytes`, waiting for the work that may
+// still read the old one.
+int grow_scratch(Device& d, uint8_t*& scratch, size_t& held, size_t bytes) {
+    if (bytes <= held) return TMH_SUCCESS;
     size_t grown = (bytes + (1u << 20) - 1) & ~(size_t)((1u << 20) - 1);
     hipError_t e = hipStreamSynchronize(d.stream);
     if (e != hipSuccess) return code(e);
-    if (d.act_scratch) (void)hipFree(d.act_scratch);
-    d.act_scratch = nullptr;
-    d.act_scratch_bytes = 0;
+    if (scratch) (void)hipFree(scratch);
+    scratch = nullptr;
+    held = 0;
     void* p = nullptr;
     e = device_malloc(&p, grown);
     if (e != hipSuccess) return e == hipErrorOutOfMemory ? TMH_ERROR_OUT_OF_MEMORY : code(e);
-    d.act_scratch = (uint8_t*)p;
-    d.act_scratch_bytes = grown;
+    scratch = (uint8_t*)p;
+    held = grown;
     return TMH_SUCCESS;
 }
+
+int ensure_scratch(Device& d, size_t bytes) { return grow_scratch(d, d.act_scratch, d.act_scratch_bytes, bytes); }
 
 size_t align256(size_t v) { return (v + 255u) & ~(size_t)255u; }
 
@@ -294,6 +302,15 @@ void note_launch(int index, int ops, bool errors) {
     if (errors) d.errors_pending.store(true);
     d.gpu_ops.fetch_add(ops);
 }
+
+Workspace::Workspace(int i, size_t bytes) : status(TMH_ERROR_NO_DEVICE), memory(nullptr), index(i) {
+    Device& d = g_devices[i];
+    d.work.lock();
+    status = grow_scratch(d, d.work_scratch, d.work_scratch_bytes, bytes);
+    memory = d.work_scratch;
+}
+
+Workspace::~Workspace() { g_devices[index].work.unlock(); }
 
 }  // namespace tmh
 

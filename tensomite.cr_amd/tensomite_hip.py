@@ -32,6 +32,9 @@ BLOCK_BYTES = {Q8_0: 34, Q4_0: 18, Q4_1: 20}
 MODES = {"auto": 0, "thread": 1, "lanes": 2, "unordered": 3, "loads": 4, "stream": 5,
          "stream_activations": 6, "matrix": 7}
 
+# Element types of a cache in pages: (ggml's number, bytes).
+CACHE_KINDS = {"F32": (0, 4), "F16": (1, 2), "BF16": (30, 2)}
+
 SUCCESS = 0
 ERROR_INVALID_VALUE = 1000
 ERROR_SHAPE = 1001
@@ -169,6 +172,11 @@ SIGNATURES = {
     "tmh_swiglu": (INT, [U64, U64, U32, U32, U32, U64]),
     "tmh_add": (INT, [U64, U64, U64, U64]),
     "tmh_argmax": (INT, [U64, U32, U32, U32, U64]),
+    "tmh_rope_write_paged": (INT, [U64, U32, U32, U32, U32, U32, U64, U64, U32, U32, U32, U32, U64, U32, U32, U64, U64,
+                                   U64, U64, U64]),
+    "tmh_attention_paged": (INT, [U64, U32, U32, U32, U32, U64, U64, U32, U32, U32, U32, U64, U32, U32, U64, U64, U32,
+                                  U32, U32, U32, F32, U64, U32]),
+    "tmh_sample": (INT, [U64, U32, U32, U32, U64, U64, U64, U64, U64, U64]),
     "tmh_llama_create": (INT, [ctypes.POINTER(LlamaConfig), ctypes.POINTER(LlamaWeights), U32, U32, U32,
                                ctypes.POINTER(U64)]),
     "tmh_llama_forward": (INT, [U64, U32, VP, U32, U32, VP]),
@@ -302,6 +310,30 @@ class Plan:
             self.destroy()
         except Exception:
             pass
+
+
+class PagedCache:
+    """Keys and values in pages, each [pages, kv_heads, page_size, width] of `kind` ("F32", "F16" or "BF16")."""
+
+    def __init__(self, kind: str, pages: int, page_size: int, kv_heads: int, width: int, keys: Buffer, values: Buffer):
+        self.kind, self.pages, self.page_size = kind, pages, page_size
+        self.kv_heads, self.width = kv_heads, width
+        self.keys, self.values = keys, values
+
+    @property
+    def code(self) -> int:
+        return CACHE_KINDS[self.kind][0]
+
+
+class PagedBatch:
+    """A call's sequences, as int32 arrays in device memory: page table [sequences, table_width], starts
+    [sequences + 1] and lengths [sequences]; no sequence has more than max_new new tokens or max_length positions."""
+
+    def __init__(self, table: Buffer, table_width: int, sequences: int, starts: Buffer, lengths: Buffer, max_new: int,
+                 max_length: int):
+        self.table, self.table_width, self.sequences = table, table_width, sequences
+        self.starts, self.lengths = starts, lengths
+        self.max_new, self.max_length = max_new, max_length
 
 
 class HIPDevice:
@@ -567,6 +599,73 @@ class HIPDevice:
             raise ShapeError("argmax: buffer too small")
         ids = ids or self.alloc(max(4 * rows, 4))
         check("tmh_argmax", self.lib.tmh_argmax(x.pointer, n, rows, n, ids.pointer))
+        return ids
+
+    # -- a cache in pages, and sampling
+    def paged_cache(self, kind: str, pages: int, page_size: int, kv_heads: int, width: int,
+                    keys: Optional[Buffer] = None, values: Optional[Buffer] = None) -> PagedCache:
+        """Keys and values in pages, in new buffers (their contents unset) unless given."""
+        if kind not in CACHE_KINDS:
+            raise DTypeError(f"{kind} is not an element type of a cache in pages")
+        size = pages * kv_heads * page_size * width * CACHE_KINDS[kind][1]
+        keys = keys or self.alloc(max(size, 4))
+        values = values or self.alloc(max(size, 4))
+        if size > min(keys.bytesize, values.bytesize):
+            raise ShapeError(f"{keys.bytesize} and {values.bytesize} bytes do not hold {pages} pages of {size} bytes")
+        return PagedCache(kind, pages, page_size, kv_heads, width, keys, values)
+
+    def paged_batch(self, table: Buffer, table_width: int, sequences: int, starts: Buffer, lengths: Buffer,
+                    max_new: int, max_length: int) -> PagedBatch:
+        """A call's sequences: page table, starts and lengths in device memory."""
+        if (sequences * table_width * 4 > table.bytesize or (sequences + 1) * 4 > starts.bytesize
+                or sequences * 4 > lengths.bytesize):
+            raise ShapeError(f"page table, starts or lengths too small for {sequences} sequences")
+        return PagedBatch(table, table_width, sequences, starts, lengths, max_new, max_length)
+
+    def rope_write_paged(self, x: Buffer, ldx: int, tokens: int, heads: int, cos: Buffer, sin: Buffer,
+                         table_rows: int, cache: PagedCache, batch: PagedBatch, q_dst: Optional[Buffer] = None) -> Buffer:
+        """RoPE of q and k and the write of k and v into the batch's pages, queued: the rotated q."""
+        row = (heads + 2 * cache.kv_heads) * cache.width
+        q_dst = q_dst or self.alloc(max(4 * tokens * heads * cache.width, 4))
+        if (tokens and ((tokens - 1) * ldx + row) * 4 > x.bytesize
+                or table_rows * cache.width * 4 > min(cos.bytesize, sin.bytesize)
+                or tokens * heads * cache.width * 4 > q_dst.bytesize):
+            raise ShapeError("rope_write_paged: buffers too small")
+        check("tmh_rope_write_paged", self.lib.tmh_rope_write_paged(
+            x.pointer, ldx, tokens, heads, cache.kv_heads, cache.width, cos.pointer, sin.pointer, table_rows,
+            cache.code, cache.pages, cache.page_size, batch.table.pointer, batch.table_width, batch.sequences,
+            batch.starts.pointer, batch.lengths.pointer, q_dst.pointer, cache.keys.pointer, cache.values.pointer))
+        return q_dst
+
+    def attention_paged(self, q: Buffer, tokens: int, heads: int, cache: PagedCache, batch: PagedBatch, scale: float,
+                        window: int = 0, sinks: int = 0, dst: Optional[Buffer] = None, ldq: Optional[int] = None,
+                        ld_dst: Optional[int] = None) -> Buffer:
+        """Attention of the batch's new tokens (q [tokens, heads, width]) over its pages, queued; with a window,
+        positions further back are hidden but for the first `sinks`."""
+        row = heads * cache.width
+        lq, ld = row if ldq is None else ldq, row if ld_dst is None else ld_dst
+        dst = dst or self.alloc(max(4 * (max(tokens - 1, 0) * ld + row), 4))
+        if tokens and (((tokens - 1) * lq + row) * 4 > q.bytesize or ((tokens - 1) * ld + row) * 4 > dst.bytesize):
+            raise ShapeError("attention_paged: buffers too small")
+        check("tmh_attention_paged", self.lib.tmh_attention_paged(
+            q.pointer, lq, tokens, heads, cache.code, cache.keys.pointer, cache.values.pointer, cache.pages,
+            cache.page_size, cache.kv_heads, cache.width, batch.table.pointer, batch.table_width, batch.sequences,
+            batch.starts.pointer, batch.lengths.pointer, batch.max_new, batch.max_length, window, sinks, scale,
+            dst.pointer, ld))
+        return dst
+
+    def sample(self, x: Buffer, rows: int, n: int, u: Buffer, temperature: Optional[Buffer] = None,
+               top_k: Optional[Buffer] = None, top_p: Optional[Buffer] = None, min_p: Optional[Buffer] = None,
+               ids: Optional[Buffer] = None, ldx: Optional[int] = None) -> Buffer:
+        """The next token of each row of logits, queued: int32 ids from u (f32 in [0, 1)) and the rows' settings."""
+        stride = n if ldx is None else ldx
+        ids = ids or self.alloc(max(4 * rows, 4))
+        arrays = [a for a in (u, temperature, top_k, top_p, min_p, ids) if a is not None]
+        if rows and ((rows - 1) * stride + n) * 4 > x.bytesize or rows * 4 > min(a.bytesize for a in arrays):
+            raise ShapeError(f"sample: buffers too small for {rows} rows of {n}")
+        address = lambda a: a.pointer if a is not None else 0  # noqa: E731
+        check("tmh_sample", self.lib.tmh_sample(x.pointer, stride, rows, n, address(temperature), address(top_k),
+                                                address(top_p), address(min_p), u.pointer, ids.pointer))
         return ids
 
     # -- timing on the library's stream

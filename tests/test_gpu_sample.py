@@ -1,0 +1,151 @@
+"""Sampling on the GPU against the definition by sorting, in 64 bits: equal ids."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+import tensomite_hip as th
+
+pytestmark = pytest.mark.gpu
+
+
+def say(*args):
+    print(*args, flush=True)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return th.HIPDevice(0)
+
+
+def settings(rng, rows):
+    """Rows of settings, every step on and off."""
+    t = rng.choice([0.0, 0.3, 0.8, 1.0, 1.7, 10.0], rows).astype(np.float32)
+    k = rng.choice([0, 1, 2, 40, 1000, 10 ** 9, -3], rows).astype(np.int32)
+    p = rng.choice([1.0, 0.0, 0.1, 0.5, 0.9, 0.999, 2.0], rows).astype(np.float32)
+    m = rng.choice([0.0, 0.01, 0.2, 1.0, 3.0], rows).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    u[::7] = 0.0
+    u[3::7] = np.float32(1.0) - np.float32(2.0 ** -24)
+    return u, t, k, p, m
+
+
+def run(dev, x, u, t=None, k=None, p=None, m=None, ldx=None, rows=None, n=None):
+    rows = x.shape[0] if rows is None else rows
+    n = x.shape[1] if n is None else n
+    up = lambda a: None if a is None else dev.from_array(a)  # noqa: E731
+    ids = dev.sample(dev.from_array(x), rows, n, up(u), temperature=up(t), top_k=up(k), top_p=up(p), min_p=up(m),
+                     ldx=ldx)
+    got = dev.to_array(ids, np.int32, rows)
+    dev.sync()
+    return got
+
+
+@pytest.mark.parametrize("n,rows", [(1, 20), (2, 40), (63, 60), (1000, 80), (4097, 60), (49152, 24), (50257, 16),
+                                    (131072, 12), (300001, 5)])
+@pytest.mark.parametrize("spread", [0.3, 3.0])
+def test_ids(dev, n, rows, spread):
+    say("sample", n, rows, spread)
+    rng = np.random.default_rng(n + int(10 * spread))
+    x = rng.normal(0, spread, (rows, n)).astype(np.float32)
+    u, t, k, p, m = settings(rng, rows)
+    got = run(dev, x, u, t, k, p, m)
+    want = [ref.sample(x[r], u[r], t[r], k[r], p[r], m[r]) for r in range(rows)]
+    assert list(got) == want
+
+
+@pytest.mark.parametrize("which", ["none", "t", "k", "p", "m"])
+def test_arrays_left_out(dev, which):
+    say("left out", which)
+    rng = np.random.default_rng(5)
+    x = rng.normal(0, 2, (30, 3001)).astype(np.float32)
+    u, t, k, p, m = settings(rng, 30)
+    given = {"t": t, "k": k, "p": p, "m": m}
+    given = {name: a for name, a in given.items() if name == which}
+    got = run(dev, x, u, **given)
+    full = {"t": np.ones(30), "k": np.zeros(30, int), "p": np.ones(30), "m": np.zeros(30), **given}
+    assert list(got) == [ref.sample(x[r], u[r], *(full[name][r] for name in "tkpm")) for r in range(30)]
+
+
+@pytest.mark.parametrize("n", [300, 1500, 9000, 40000])
+def test_ties(dev, n):
+    # few values many times over, and one value only: equal candidates by rising index
+    say("ties", n)
+    rng = np.random.default_rng(n)
+    rows = 36
+    x = rng.integers(-3, 4, (rows, n)).astype(np.float32)
+    x[::3] = np.where(rng.random((12, n)) < 0.5, np.float32(0.0), np.float32(-0.0))
+    x[1::3] = np.float32(2.5) + rng.integers(0, 3, (12, n)).astype(np.float32) * np.float32(2.0 ** -22)
+    u, t, k, p, m = settings(rng, rows)
+    k = np.where(k > 2, rng.integers(1, n + 1, rows), k).astype(np.int32)
+    got = run(dev, x, u, t, k, p, m)
+    assert list(got) == [ref.sample(x[r], u[r], t[r], k[r], p[r], m[r]) for r in range(rows)]
+
+
+def test_many_close_values(dev):
+    # one bin of the histogram with more values than are put in order at once, all different
+    say("close")
+    rng = np.random.default_rng(8)
+    rows, n = 12, 30000
+    x = (np.float32(1.0) + rng.permutation(n).astype(np.float32) * np.float32(2.0 ** -23))[None].repeat(rows, 0)
+    x[:, 0] = -30.0
+    x[:, 1] = 1.0 + 2.0 ** -6
+    u = rng.random(rows).astype(np.float32)
+    t = np.full(rows, 1.0, np.float32)
+    k = np.array([0, 5, 3000, 20000] * 3, np.int32)
+    p = np.array([1.0, 0.5, 0.9] * 4, np.float32)
+    got = run(dev, x, u, t, k, p)
+    assert list(got) == [ref.sample(x[r], u[r], t[r], k[r], p[r]) for r in range(rows)]
+
+
+def test_masked_and_odd_logits(dev):
+    say("masked")
+    rng = np.random.default_rng(9)
+    n = 2000
+    x = rng.normal(0, 2, (12, n)).astype(np.float32)
+    x[0, 5:] = -np.inf
+    x[1] = -np.inf
+    x[1, 1234] = -80.0
+    x[2] = -np.inf                          # nothing left: the greedy choice
+    x[3] = np.nan
+    x[4, ::2] = np.nan
+    x[5, 17] = np.inf
+    x[6, [100, 900]] = np.inf
+    x[7] = np.finfo(np.float32).min         # masks of the type's lowest value
+    x[7, 50:60] = 1.0
+    x[8] = np.finfo(np.float32).min
+    x[9] = np.finfo(np.float32).max
+    x[10, 0] = np.nan
+    x[11] *= 1e30
+    for trial in range(6):
+        u, t, k, p, m = settings(rng, 12)
+        got = run(dev, x, u, t, k, p, m)
+        assert list(got) == [ref.sample(x[r], u[r], t[r], k[r], p[r], m[r]) for r in range(12)]
+
+
+def test_random_numbers_out_of_range(dev):
+    say("range")
+    x = np.array([[0.0, 3.0, 1.0, 2.0]] * 4, np.float32)
+    got = run(dev, x, np.array([1.0, 7.0, -1.0, np.nan], np.float32))
+    assert list(got) == [0, 0, 1, 0]  # the last that stays, the last, the first, the last
+    got = run(dev, x, np.array([1.0, 0.99, 0.99, 0.99], np.float32), k=np.array([2, 2, 3, 1], np.int32))
+    assert list(got) == [3, 3, 2, 1]
+
+
+def test_strided_rows_and_the_same_ids_again(dev):
+    say("strided")
+    rng = np.random.default_rng(11)
+    x = rng.normal(0, 2, (9, 5003)).astype(np.float32)
+    u, t, k, p, m = settings(rng, 9)
+    got = run(dev, x, u, t, k, p, m, ldx=5003, rows=9, n=4999)
+    assert list(got) == [ref.sample(x[r, :4999], u[r], t[r], k[r], p[r], m[r]) for r in range(9)]
+    for _ in range(3):
+        assert list(run(dev, x, u, t, k, p, m, ldx=5003, rows=9, n=4999)) == list(got)
+
+
+def test_frequencies(dev):
+    # 4096 even steps of u over one row: each token as often as its weight says, to one step
+    say("frequencies")
+    x = np.tile(np.log(np.array([0.5, 0.25, 0.15, 0.1], np.float32)), (4096, 1))
+    u = ((np.arange(4096) + 0.5) / 4096).astype(np.float32)
+    counts = np.bincount(run(dev, x, u), minlength=4)
+    assert np.abs(counts - 4096 * np.array([0.5, 0.25, 0.15, 0.1])).max() <= 1.0

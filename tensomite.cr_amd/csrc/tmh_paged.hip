@@ -13,6 +13,7 @@
 #include "tmh_device.h"
 #include "tmh_internal.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace tmh {
@@ -186,16 +187,27 @@ __global__ __launch_bounds__(256) void k_rope_write_paged(WritePaged a) {
 struct AttendPaged {
     Paged p;
     const float* q;
-    uint32_t ldq, heads, group;
+    uint32_t ldq, heads;
+    Divider group;  // by the query heads of a kv head
     const void* keys;
     const void* values;
     uint32_t window, sinks;
     float scale;  // times log2 e
     float* dst;
     uint32_t ld_dst;
+    // Tiles of keys that one workgroup takes; where a row has more, its parts
+    // (unscaled outputs; the reference score and the sum of weights) go to
+    // part and k_attend_join joins them. `splits` parts a row have room.
+    // The parts of few rows stand by sequence, kv head and row, `room` rows
+    // each; those of other rows (room 0) by token and head.
+    uint32_t share, splits, room;
+    float* part;
+    float2* part_sums;
 };
 
-constexpr uint32_t KEYS = 64;  // positions of a tile of keys
+constexpr uint32_t KEYS = 64;      // positions of a tile of keys
+constexpr uint32_t FEW_TILE = 16;  // query rows of a tile of few rows
+constexpr uint32_t FEW_ROWS = 32;  // the most query rows of a kv head that are few
 
 // The tiles of keys that positions [lo, hi] see: `early` of the sinks, then
 // those from the window's first, `from`, on.
@@ -206,11 +218,14 @@ struct Span {
     }
 };
 
+__device__ __forceinline__ uint32_t window_start(const AttendPaged& a, uint32_t pos) {
+    return a.window && pos >= a.window ? pos - a.window + 1u : 0u;
+}
+
 __device__ __forceinline__ Span span_of(const AttendPaged& a, uint32_t lo, uint32_t hi) {
     Span s;
-    const uint32_t low = a.window && lo >= a.window ? lo - a.window + 1u : 0u;
-    s.from = low / KEYS * KEYS;
-    s.early = min((a.sinks + KEYS - 1u) / KEYS, s.from / KEYS);
+    s.from = window_start(a, lo) / KEYS * KEYS;
+    s.early = min(a.sinks / KEYS + (a.sinks % KEYS ? 1u : 0u), s.from / KEYS);
     s.tiles = s.early + (hi - s.from) / KEYS + 1u;
     return s;
 }
@@ -219,28 +234,84 @@ __device__ __forceinline__ bool sees(const AttendPaged& a, uint32_t pos, uint32_
     return j <= pos && (a.window == 0u || pos - j < a.window || j < a.sinks);
 }
 
-// One query row by one workgroup: the plain form, a thread per key and
-// quarter of its columns for the scores, a thread per column for the values.
+// A tile of a sequence's query rows of one kv head: row r is new token
+// r / group, query head kh * group + r % group.
+struct Rows {
+    uint32_t s, kh, first, count;  // the tile's first row, and rows
+    Sequence sq;
+    uint32_t lo, hi;  // positions of its first and last row
+    Span span;
+    uint32_t parts, begin, end;  // its parts, and the tiles of keys of this one
+
+    __device__ __forceinline__ uint32_t token(const AttendPaged& a, uint32_t r) const {
+        return sq.first + a.group.divide(r);
+    }
+    __device__ __forceinline__ uint32_t head(const AttendPaged& a, uint32_t r) const {
+        return kh * a.group.d + r - a.group.divide(r) * a.group.d;
+    }
+    __device__ __forceinline__ uint32_t position(const AttendPaged& a, uint32_t r) const {
+        return sq.length - sq.count + a.group.divide(r);
+    }
+    // The rows from `from` on (a multiple of `size`), `size` at most; part
+    // `part` of theirs. False when there are none.
+    __device__ __forceinline__ bool set(const AttendPaged& a, uint32_t from, uint32_t size, uint32_t part) {
+        const uint32_t all = sq.count * a.group.d;
+        if (from >= all) return false;
+        first = from;
+        count = min(size, all - from);
+        lo = position(a, from);
+        hi = position(a, from + count - 1u);
+        span = span_of(a, lo, hi);
+        parts = (span.tiles + a.share - 1u) / a.share;
+        if (part >= parts) return false;
+        // even parts, so that none is a remainder
+        begin = (uint32_t)((uint64_t)span.tiles * part / parts);
+        end = (uint32_t)((uint64_t)span.tiles * (part + 1u) / parts);
+        return true;
+    }
+    // Where row r's parts stand.
+    __device__ __forceinline__ size_t place(const AttendPaged& a, uint32_t r) const {
+        return (a.room ? ((size_t)s * a.p.kv_heads + kh) * a.room + r : (size_t)token(a, r) * a.heads + head(a, r)) *
+               a.splits;
+    }
+    // Whether position pos sees any key of the part.
+    __device__ __forceinline__ bool sees_any(const AttendPaged& a, uint32_t pos) const {
+        for (uint32_t tile = begin; tile < end; ++tile) {
+            const uint32_t k = span.key(tile);
+            if (k <= pos && (a.window == 0u || pos < k + KEYS || pos - (k + KEYS - 1u) < a.window || k < a.sinks)) return true;
+        }
+        return false;
+    }
+    // The cache row to read for position j: j's, or where no row of the tile
+    // sees j that of the last position, so that pages of hidden positions
+    // alone are never touched; a page out of range is reported, and page 0's.
+    __device__ __forceinline__ uint32_t cache_row_for(const AttendPaged& a, uint32_t j) const {
+        const bool some = j <= hi && (j >= window_start(a, lo) || j < a.sinks);
+        uint32_t row = 0;
+        cache_row(a.p, s, some ? j : hi, kh, row);
+        return row;
+    }
+};
+
+// The plain form of one query row over the tiles of keys [begin, end), by a
+// workgroup of 256 threads: a thread per key and quarter of its columns for
+// the scores, a thread per column for the values; hidden positions are not
+// read. The kernels below give it the rows whose results are not finite: what
+// is not a number or not finite among hidden positions reaches the
+// matrix cores' sums (0 times NaN), as do infinities split into parts.
+// Returns column threadIdx.x of the sums, with the reference score and the
+// sum of weights.
 template <uint32_t KIND>
-__global__ __launch_bounds__(256) void k_attend_row(AttendPaged a) {
+__device__ __forceinline__ float plain_row(const AttendPaged& a, uint32_t s, uint32_t kh, uint32_t pos,
+                                                     const float* q, const Span& span, uint32_t begin, uint32_t end,
+                                                     float& top, float& total) {
     typedef typename Element<KIND>::type T;
     __shared__ float weight[KEYS];
     __shared__ uint32_t rows[KEYS];
-    const uint32_t t = blockIdx.x / a.heads, h = blockIdx.x % a.heads, kh = h / a.group;
-    const uint32_t s = sequence_of(a.p, t);
-    if (s >= a.p.sequences || (int32_t)t < a.p.starts[0]) return;
-    Sequence sq;
-    const bool fits = read_sequence(a.p, s, sq);
-    const uint32_t i = t - sq.first;
-    if (!fits || i >= sq.count) {
-        if (threadIdx.x == 0 && h == 0) report(a.p.errors, (int32_t)s, (int32_t)a.p.sequences);
-        return;
-    }
-    const uint32_t pos = sq.length - sq.count + i, width = a.p.width, quarter = width / 4u;
-    const float* q = a.q + (size_t)t * a.ldq + h * width;
-    const Span span = span_of(a, pos, pos);
-    float top = -INFINITY, total = 0.0f, out = 0.0f;
-    for (uint32_t tile = 0; tile < span.tiles; ++tile) {
+    const uint32_t width = a.p.width, quarter = width / 4u;
+    float out = 0.0f;
+    top = -INFINITY, total = 0.0f;
+    for (uint32_t tile = begin; tile < end; ++tile) {
         const uint32_t j = span.key(tile) + threadIdx.x / 4u;
         float score = 0.0f;
         uint32_t row = 0;
@@ -255,17 +326,18 @@ __global__ __launch_bounds__(256) void k_attend_row(AttendPaged a) {
         __syncthreads();  // the last tile's weights have been read
         if (threadIdx.x % 4u == 0) {
             weight[threadIdx.x / 4u] = seen ? score : -INFINITY;
-            rows[threadIdx.x / 4u] = seen ? row : 0xffffffffu;
+            rows[threadIdx.x / 4u] = seen ? row : ~0u;
         }
         __syncthreads();
-        float best = weight[threadIdx.x & 63u];
-        const float mine = best;
+        const float mine = weight[threadIdx.x & 63u];
+        const bool is = rows[threadIdx.x & 63u] != ~0u;
+        float best = mine;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) best = fmaxf(best, __shfl_xor(best, d, 64));
         const float higher = fmaxf(top, best);
         const float ref = higher == -INFINITY ? 0.0f : higher;
         const float keep = __builtin_amdgcn_exp2f(top - ref);
-        float e = rows[threadIdx.x & 63u] != 0xffffffffu ? __builtin_amdgcn_exp2f(mine - ref) : 0.0f;
+        const float e = is ? __builtin_amdgcn_exp2f(mine - ref) : 0.0f;
         float sum = e;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
@@ -277,9 +349,470 @@ __global__ __launch_bounds__(256) void k_attend_row(AttendPaged a) {
         out *= keep;
         if (threadIdx.x < width)
             for (uint32_t k = 0; k < KEYS; ++k)
-                if (rows[k] != 0xffffffffu) out += weight[k] * (float)((const T*)a.values)[(size_t)rows[k] * width + threadIdx.x];
+                if (rows[k] != ~0u) out += weight[k] * (float)((const T*)a.values)[(size_t)rows[k] * width + threadIdx.x];
     }
-    if (threadIdx.x < width) a.dst[(size_t)t * a.ld_dst + h * width + threadIdx.x] = out / total;
+    return out;
+}
+
+// Writes a row's result, or its part: column c of `width`.
+__device__ __forceinline__ void put_column(const AttendPaged& a, const Rows& w, uint32_t r, uint32_t part, uint32_t c,
+                                           float sum, float top, float total) {
+    if (w.parts == 1u) {
+        a.dst[(size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * a.p.width + c] = sum / total;
+        return;
+    }
+    const size_t at = w.place(a, r) + part;
+    a.part[at * a.p.width + c] = sum;
+    if (c == 0) a.part_sums[at] = make_float2(top, total);
+}
+
+// The tile's rows whose bit is set in `which`, by the plain form.
+template <uint32_t KIND>
+__device__ __forceinline__ void plain_rows(const AttendPaged& a, const Rows& w, uint32_t part, const uint32_t* which) {
+    for (uint32_t i = 0; i < w.count; ++i) {
+        if (!(which[i / 32u] >> i % 32u & 1u)) continue;
+        const uint32_t r = w.first + i;
+        float top, total;
+        const float* q = a.q + (size_t)w.token(a, r) * a.ldq + w.head(a, r) * a.p.width;
+        const float sum = plain_row<KIND>(a, w.s, w.kh, w.position(a, r), q, w.span, w.begin, w.end, top, total);
+        if (threadIdx.x < a.p.width) put_column(a, w, r, part, threadIdx.x, sum, top, total);
+    }
+}
+
+// One query row by one workgroup.
+template <uint32_t KIND>
+__global__ __launch_bounds__(256) void k_attend_row(AttendPaged a) {
+    const uint32_t t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    Rows w;
+    w.s = sequence_of(a.p, t);
+    w.kh = a.group.divide(h);
+    if (w.s >= a.p.sequences || (int32_t)t < a.p.starts[0]) return;
+    const bool fits = read_sequence(a.p, w.s, w.sq);
+    const uint32_t i = t - w.sq.first;
+    if (!fits || i >= w.sq.count) {
+        if (threadIdx.x == 0 && h == 0) report(a.p.errors, (int32_t)w.s, (int32_t)a.p.sequences);
+        return;
+    }
+    if (w.sq.count * a.group.d <= FEW_ROWS) return;  // k_attend_few's
+    if (!w.set(a, i * a.group.d + h - w.kh * a.group.d, 1, 0)) return;
+    w.parts = 1, w.end = w.span.tiles;
+    const uint32_t first = 1;
+    plain_rows<KIND>(a, w, 0, &first);
+}
+
+// ------------------------------------------------------- on the matrix cores
+//
+// The matrix cores multiply 16-bit numbers exactly and add in f32, so f32
+// accuracy takes numbers in parts: an f32 number is the sum of three bf16
+// ones (its 24 bits cut in eights, exactly), or of two f16 ones to 2^-22 of
+// it. An F16 or BF16 cache is one part as it stands; the queries and the
+// weights of the softmax have PARTS parts of its type, and an F32 cache three
+// of bf16, of whose products with theirs those down to 2^-16 of the first are
+// taken (three more would add 2^-24 and less).
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+template <uint32_t KIND>
+struct Split {
+    static constexpr uint32_t PARTS = KIND == TMH_CACHE_F16 ? 2 : 3;        // of f32 numbers
+    static constexpr uint32_t CACHE_PARTS = KIND == TMH_CACHE_F32 ? 3 : 1;  // of the cache's
+    static constexpr uint32_t BYTES = KIND == TMH_CACHE_F32 ? 4 : 2;
+};
+
+// Eight numbers of each part, as a matrix operand holds them.
+template <uint32_t N>
+struct Operand {
+    u32x4 part[N];
+};
+
+// Parts of the numbers v0 and v1, at pair `at` of the operand. Cutting rounds
+// toward zero; what it leaves goes to the next part. f16 (v below 65536): two
+// times 11 bits, at least 2^-25 absolute.
+template <uint32_t KIND>
+__device__ __forceinline__ void split_pair(Operand<Split<KIND>::PARTS>& o, int at, float v0, float v1) {
+    if constexpr (KIND == TMH_CACHE_F16) {
+        const float h0 = __uint_as_float(__float_as_uint(v0) & 0xffffe000u);
+        const float h1 = __uint_as_float(__float_as_uint(v1) & 0xffffe000u);
+        o.part[0][at] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(h0, h1));
+        o.part[1][at] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v0 - h0, v1 - h1));
+    } else {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const uint32_t w0 = __float_as_uint(v0), w1 = __float_as_uint(v1);
+            o.part[p][at] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+            v0 -= __uint_as_float(w0 & 0xffff0000u);
+            v1 -= __uint_as_float(w1 & 0xffff0000u);
+        }
+    }
+}
+
+template <uint32_t KIND>
+__device__ __forceinline__ f32x4 multiply16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (KIND == TMH_CACHE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The products of a cache operand's parts and another's, smallest first.
+template <uint32_t KIND>
+__device__ __forceinline__ f32x4 multiply_parts16(const Operand<Split<KIND>::CACHE_PARTS>& a,
+                                                  const Operand<Split<KIND>::PARTS>& b, f32x4 c) {
+    constexpr int LAST = (int)Split<KIND>::PARTS - 1;
+#pragma unroll
+    for (int order = LAST; order >= 0; --order)
+#pragma unroll
+        for (int p = 0; p < (int)Split<KIND>::CACHE_PARTS; ++p)
+            if (order - p >= 0) c = multiply16<KIND>(a.part[p], b.part[order - p], c);
+    return c;
+}
+
+// Scores are compared with a row's reference, the highest when it was last
+// set; weights are 2^(score - reference + HEADROOM), and the reference is set
+// anew once a score passes it by SLACK. Weights stay below 2^(HEADROOM + SLACK),
+// within f16, and those down to 2^-24 of the reference's have all their bits.
+constexpr float HEADROOM = 6.0f, SLACK = 8.0f;
+constexpr float NO_REFERENCE = -3.0e38f;
+
+// A power of two that brings the largest magnitude of a row of f16 parts to
+// 2^13 .. 2^14.
+__device__ __forceinline__ float power_for(float largest) {
+    const int e = (int)(__float_as_uint(largest) >> 23) - 127;
+    if (largest == 0.0f || e > 127) return 1.0f;
+    return __uint_as_float((uint32_t)(min(13 - e, 126) + 127) << 23);
+}
+
+// ---------------------------------------------------------------- few query rows
+
+// Decode steps and chunks of a few tokens: up to FEW_TILE query rows of a kv
+// head against a share of the keys. Reading the cache bounds it, so the four
+// waves take 32 positions each in turn, nothing shared: keys go from memory to
+// the operand's registers, values through the wave's own LDS (direct loads,
+// then transposed reads), both loaded a step ahead. Scores are taken
+// transposed, keys down and queries across: a lane then holds weights of one
+// query and of eight keys, which is what the second product wants of it, with
+// the keys in the order 4g..4g+3, 16+4g..16+4g+3 for lane group g.
+template <uint32_t KIND, uint32_t W>
+struct Few {
+    static constexpr uint32_t BYTES = Split<KIND>::BYTES;
+    static constexpr uint32_t CHUNKS = W * BYTES / 16u;         // 16-byte chunks of a row
+    static constexpr uint32_t STAGE = 32u * W * BYTES;          // values of one step
+    static constexpr uint32_t STAGES = STAGE <= 16384u ? 2 : 1;  // ahead, where four waves' fit the LDS
+    static constexpr uint32_t LOADS = STAGE / 1024u;
+    static constexpr uint32_t EIGHT = BYTES / 2u;               // 16-byte pieces of eight numbers
+    static constexpr uint32_t STEPS = W / 32u;                  // of the score's product
+    static constexpr uint32_t OUT = 4u * FEW_TILE * (W + 4u) * 4u;
+    static constexpr uint32_t LDS = 4u * STAGE * STAGES > OUT ? 4u * STAGE * STAGES : OUT;
+    // Where a chunk of a row stands in it, so that what is read at once falls
+    // on different banks: four rows by four lane groups of one column's 64
+    // bytes (f32), or sixteen rows of 32 bytes (f16, bf16).
+    static __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t chunk, uint32_t row) {
+        return BYTES == 4u ? chunk ^ ((row >> 2 & (CHUNKS / 4u - 1u) & 3u) << 2) : chunk ^ (row & (CHUNKS - 1u) & 7u);
+    }
+};
+
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_tiles) {
+    typedef Few<KIND, W> F;
+    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ float tops[4][FEW_TILE], totals[4][FEW_TILE];
+    __shared__ uint32_t redo;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, group = lane >> 4;
+    Rows w;
+    uint32_t b = blockIdx.x;
+    w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
+    const uint32_t row_tile = b % row_tiles;
+    b /= row_tiles;
+    w.s = b % a.p.sequences;
+    const uint32_t part = b / a.p.sequences;
+    if (!read_sequence(a.p, w.s, w.sq)) {
+        if (b < a.p.sequences && w.kh == 0 && row_tile == 0 && threadIdx.x == 0)
+            report(a.p.errors, (int32_t)w.s, (int32_t)a.p.sequences);
+        return;
+    }
+    if (w.sq.count * a.group.d > FEW_ROWS || !w.set(a, row_tile * FEW_TILE, FEW_TILE, part)) return;
+    const uint32_t width = a.p.width;
+
+    // this lane's query: rows past the tile's repeat its last
+    const uint32_t r = w.first + min(col, w.count - 1u);
+    const uint32_t pos = w.position(a, r);
+    const float* q = a.q + (size_t)w.token(a, r) * a.ldq + w.head(a, r) * width;
+    Operand<NP> query[F::STEPS];
+    float power = 1.0f, undo = 1.0f;
+    {
+        float v[F::STEPS][8];
+        float largest = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < F::STEPS; ++k) {
+            const uint32_t c = k * 32u + group * 8u;
+            const Four* from = reinterpret_cast<const Four*>(q + (c < width ? c : 0u));
+            const Four lo = from[0], hi = from[1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[k][j] = j < 4 ? lo.v[j & 3] : hi.v[j & 3];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < F::STEPS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[k][j] = k * 32u + group * 8u < width ? v[k][j] * a.scale : 0.0f;
+                largest = fmaxf(largest, fabsf(v[k][j]));
+            }
+        if (KIND == TMH_CACHE_F16) {
+            largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
+            largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+            power = power_for(largest);
+            undo = 1.0f / power;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < F::STEPS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) split_pair<KIND>(query[k], j / 2, v[k][j] * power, v[k][j + 1] * power);
+    }
+
+    uint8_t* stage = lds + wave * F::STAGE * F::STAGES;
+    const uint32_t stage_at = lds_address(stage);
+    const size_t row_bytes = (size_t)width * F::BYTES;
+    // step i of this wave: 32 positions, two steps a tile of keys
+    const uint32_t steps = 2u * (w.end - w.begin);
+    const auto first_key = [&](uint32_t i) { return w.span.key(w.begin + i / 2u) + (i & 1u) * 32u; };
+    // the step's keys, 8 columns of rows col and 16 + col each (where a row is
+    // narrower than W its first columns stand in, taken for 0); its values
+    const auto load = [&](uint32_t i, uint32_t buffer, u32x4 (&key)[2][F::STEPS][F::EIGHT]) {
+        const uint32_t mine = w.cache_row_for(a, first_key(i) + (lane & 31u));
+#pragma unroll
+        for (uint32_t t = 0; t < 2u; ++t) {
+            const uint8_t* from = (const uint8_t*)a.keys + (size_t)__shfl(mine, t * 16u + col, 64) * row_bytes;
+#pragma unroll
+            for (uint32_t k = 0; k < F::STEPS; ++k) {
+                const uint32_t c = k * 32u + group * 8u;
+#pragma unroll
+                for (uint32_t e = 0; e < F::EIGHT; ++e)
+                    key[t][k][e] = *(const u32x4*)(from + (c < width ? c : 0u) * F::BYTES + e * 16u);
+            }
+        }
+#pragma unroll
+        for (uint32_t l = 0; l < F::LOADS; ++l) {
+            const uint32_t slot = l * 64u + lane, row = slot / F::CHUNKS;
+            const uint32_t at = F::swizzle(slot % F::CHUNKS, row) * 16u;
+            const uint8_t* from = (const uint8_t*)a.values + (size_t)__shfl(mine, row, 64) * row_bytes;
+            lds_load16(from + (at < row_bytes ? at : 0u), stage_at + buffer * F::STAGE + l * 1024u);
+        }
+    };
+
+    float ref = NO_REFERENCE, total = 0.0f;
+    f32x4 out[W / 16u];
+#pragma unroll
+    for (uint32_t d = 0; d < W / 16u; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4 key[2][F::STEPS][F::EIGHT], next[2][F::STEPS][F::EIGHT];
+    if (F::STAGES == 2u && wave < steps) load(wave, 0, key);
+    uint32_t buffer = 0;
+    for (uint32_t i = wave; i < steps; i += 4u) {
+        if (F::STAGES == 1u) load(i, 0, key);
+        wait_vm_lds<0>();
+        asm volatile("" ::: "memory");
+        const bool more = F::STAGES == 2u && i + 4u < steps;
+        if (more) load(i + 4u, buffer ^ 1u, next);
+
+        f32x4 score[2];
+#pragma unroll
+        for (uint32_t t = 0; t < 2u; ++t) {
+            score[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t k = 0; k < F::STEPS; ++k) {
+                Operand<CP> o;
+                if (width < W && k * 32u + group * 8u >= width)
+#pragma unroll
+                    for (uint32_t e = 0; e < F::EIGHT; ++e) key[t][k][e] = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (KIND == TMH_CACHE_F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        split_pair<KIND>(o, j, __uint_as_float(key[t][k][j / 2][j % 2 * 2]),
+                                         __uint_as_float(key[t][k][j / 2][j % 2 * 2 + 1]));
+                } else {
+                    o.part[0] = key[t][k][0];
+                }
+                score[t] = multiply_parts16<KIND>(o, query[k], score[t]);
+            }
+        }
+        const uint32_t k0 = first_key(i);
+        const bool whole = k0 + 31u <= w.lo && (a.window == 0u || w.hi - k0 < a.window || k0 + 31u < a.sinks);
+        float best = -INFINITY;
+#pragma unroll
+        for (uint32_t t = 0; t < 2u; ++t)
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+                if (KIND == TMH_CACHE_F16) score[t][j] *= undo;
+                if (!whole && !sees(a, pos, k0 + t * 16u + group * 4u + j)) score[t][j] = -INFINITY;
+                best = fmaxf(best, score[t][j]);
+            }
+        if (__any(best > ref + SLACK)) {
+            best = fmaxf(best, __shfl_xor(best, 16, 64));
+            best = fmaxf(best, __shfl_xor(best, 32, 64));
+            if (best > ref + SLACK) {
+                const float keep = __builtin_amdgcn_exp2f(ref - best);
+                ref = best;
+                total *= keep;
+#pragma unroll
+                for (uint32_t d = 0; d < W / 16u; ++d) out[d] *= keep;
+            }
+        }
+        const float zero = ref - HEADROOM;
+        Operand<NP> weight;
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t t = 0; t < 2u; ++t) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; ++j) {
+                score[t][j] = __builtin_amdgcn_exp2f(score[t][j] - zero);
+                sum += score[t][j];
+            }
+            split_pair<KIND>(weight, (int)t * 2, score[t][0], score[t][1]);
+            split_pair<KIND>(weight, (int)t * 2 + 1, score[t][2], score[t][3]);
+        }
+        total += sum;
+        const uint8_t* from = stage + buffer * F::STAGE;
+#pragma unroll
+        for (uint32_t d = 0; d < W / 16u; ++d) {
+            Operand<CP> o;
+            if constexpr (KIND == TMH_CACHE_F32) {
+                float v[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    const uint32_t row = group * 4u + j % 4u + j / 4u * 16u;
+                    v[j] = *(const float*)(from + row * W * 4u + F::swizzle(d * 4u + col / 4u, row) * 16u + col % 4u * 4u);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) split_pair<KIND>(o, j / 2, v[j], v[j + 1]);
+            } else {
+                // 4 rows of 16 columns a lane group, turned: 4 rows of a column a lane
+                const uint32_t row = group * 4u + col / 4u;
+                const uint32_t at = stage_at + buffer * F::STAGE + row * W * 2u +
+                                    F::swizzle(d * 2u + col % 4u / 2u, row) * 16u + col % 2u * 8u;
+                const uint64_t early = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at));
+                const uint64_t late = __builtin_bit_cast(
+                    uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + 16u * W * 2u)));
+                o.part[0] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
+            }
+            out[d] = multiply_parts16<KIND>(o, weight, out[d]);
+        }
+        if (more) {
+#pragma unroll
+            for (uint32_t t = 0; t < 2u; ++t)
+#pragma unroll
+                for (uint32_t k = 0; k < F::STEPS; ++k)
+#pragma unroll
+                    for (uint32_t e = 0; e < F::EIGHT; ++e) key[t][k][e] = next[t][k][e];
+            buffer ^= 1u;
+        }
+    }
+
+    // the four waves' sums, brought to one reference and added
+    total += __shfl_xor(total, 16, 64);
+    total += __shfl_xor(total, 32, 64);
+    if (group == 0) tops[wave][col] = ref, totals[wave][col] = total;
+    if (threadIdx.x == 0) redo = 0;
+    __syncthreads();
+    {
+        const float top = fmaxf(fmaxf(tops[0][col], tops[1][col]), fmaxf(tops[2][col], tops[3][col]));
+        const float keep = __builtin_amdgcn_exp2f(ref - top);
+        float* to = (float*)lds + (wave * FEW_TILE + col) * (W + 4u) + group * 4u;
+#pragma unroll
+        for (uint32_t d = 0; d < W / 16u; ++d) *(f32x4*)(to + d * 16u) = out[d] * keep;
+    }
+    __syncthreads();
+    const uint32_t c = threadIdx.x % W;
+    for (uint32_t i = threadIdx.x / W; i < w.count; i += 256u / W) {
+        if (c >= width) break;
+        const float top = fmaxf(fmaxf(tops[0][i], tops[1][i]), fmaxf(tops[2][i], tops[3][i]));
+        float sum = 0.0f, all = 0.0f;
+#pragma unroll
+        for (uint32_t v = 0; v < 4u; ++v) {
+            sum += ((const float*)lds)[(v * FEW_TILE + i) * (W + 4u) + c];
+            all += totals[v][i] * __builtin_amdgcn_exp2f(tops[v][i] - top);
+        }
+        const uint32_t row = w.first + i;
+        if (!(fabsf(sum) < INFINITY) || !(all < INFINITY) || (all == 0.0f && w.sees_any(a, w.position(a, row))))
+            atomicOr(&redo, 1u << i);
+        put_column(a, w, row, part, c, sum, top - HEADROOM, all);
+    }
+    __syncthreads();
+    const uint32_t again = redo;
+    if (again) plain_rows<KIND>(a, w, part, &again);
+}
+
+// Joins the parts of a row: each brought to the highest reference, a wave
+// every fourth part.
+__global__ __launch_bounds__(256) void k_attend_join(AttendPaged a) {
+    __shared__ float sums[4][256];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, width = a.p.width;
+    Rows w;
+    uint32_t b = blockIdx.x;
+    const uint32_t r = b % a.room;
+    b /= a.room;
+    w.kh = b % a.p.kv_heads;
+    w.s = b / a.p.kv_heads;
+    if (!read_sequence(a.p, w.s, w.sq)) return;
+    const uint32_t rows = w.sq.count * a.group.d;
+    if (rows > FEW_ROWS || r >= rows || !w.set(a, r / FEW_TILE * FEW_TILE, FEW_TILE, 0) || w.parts == 1u) return;
+    const size_t at = w.place(a, r);
+    float top = -INFINITY;
+    for (uint32_t z = lane; z < w.parts; z += 64u) top = fmaxf(top, a.part_sums[at + z].x);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f;
+    for (uint32_t z = lane; z < w.parts; z += 64u) {
+        const float2 one = a.part_sums[at + z];
+        total += one.y * __builtin_amdgcn_exp2f(one.x - ref);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, 64);
+    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t z = wave; z < w.parts; z += 4u) {
+        const float keep = __builtin_amdgcn_exp2f(a.part_sums[at + z].x - ref);
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+            if (lane + i * 64u < width) out[i] += a.part[(at + z) * width + lane + i * 64u] * keep;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) sums[wave][lane + i * 64u] = out[i];
+    __syncthreads();
+    const uint32_t c = threadIdx.x;
+    if (c < width)
+        a.dst[(size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width + c] =
+            (sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]) / total;
+}
+
+template <uint32_t KIND, uint32_t W>
+void launch_few(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipStream_t stream) {
+    constexpr uint32_t lds = Few<KIND, W>::LDS;
+    TMH_LAUNCH((k_attend_few<KIND, W>), dim3(grid), dim3(256), lds, stream, a, row_tiles);
+}
+
+template <uint32_t KIND>
+void launch_few_of(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipStream_t stream) {
+    if (a.p.width <= 32u)
+        launch_few<KIND, 32>(a, row_tiles, grid, stream);
+    else if (a.p.width <= 64u)
+        launch_few<KIND, 64>(a, row_tiles, grid, stream);
+    else if (a.p.width <= 128u)
+        launch_few<KIND, 128>(a, row_tiles, grid, stream);
+    else
+        launch_few<KIND, 256>(a, row_tiles, grid, stream);
+}
+
+// Tiles of keys that a row tile of `tokens` new tokens sees, at most.
+uint64_t most_tiles(const AttendPaged& a, uint32_t tokens) {
+    const uint64_t all = ((uint64_t)a.p.max_length + KEYS - 1u) / KEYS;
+    if (a.window == 0u) return all;
+    return std::min<uint64_t>(all, ((uint64_t)a.sinks + KEYS - 1u) / KEYS + ((uint64_t)a.window + tokens + KEYS) / KEYS + 1u);
 }
 
 int check_paged(uint32_t tokens, uint32_t kind, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t width,
@@ -350,18 +883,53 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
         return TMH_ERROR_INVALID_VALUE;
     DeviceContext ctx;
     if ((err = device_context(&ctx, true)) != TMH_SUCCESS) return err;
+    const uint32_t group = heads / kv_heads;
     AttendPaged a{{(const int32_t*)page_table, (const int32_t*)starts, (const int32_t*)lengths, table_width, sequences,
                    tokens, max_new, max_length, pages, kv_heads, width, Divider(page_size), ctx.errors},
-                  (const float*)q, ldq, heads, heads / kv_heads, (const void*)keys, (const void*)values, window, sinks,
-                  (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst};
-    const dim3 grid(tokens * heads);
-    if (kind == TMH_CACHE_F32)
-        TMH_LAUNCH(k_attend_row<TMH_CACHE_F32>, grid, dim3(256), 0, ctx.stream, a);
-    else if (kind == TMH_CACHE_F16)
-        TMH_LAUNCH(k_attend_row<TMH_CACHE_F16>, grid, dim3(256), 0, ctx.stream, a);
-    else
-        TMH_LAUNCH(k_attend_row<TMH_CACHE_BF16>, grid, dim3(256), 0, ctx.stream, a);
-    const hipError_t e = hipGetLastError();
+                  (const float*)q, ldq, heads, Divider(group), (const void*)keys, (const void*)values, window, sinks,
+                  (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst, 0, 1, 0, nullptr, nullptr};
+    // few rows: shares of the keys such that four workgroups a compute unit
+    // have one each, of at least a step for each of their waves
+    a.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, (uint64_t)max_new * group);
+    const uint32_t row_tiles = (a.room + FEW_TILE - 1u) / FEW_TILE;
+    const uint64_t tiles = std::max<uint64_t>(1u, most_tiles(a, FEW_ROWS));
+    const uint64_t groups = (uint64_t)sequences * kv_heads * row_tiles;
+    if (groups > 0x7fffffffull) return TMH_ERROR_SHAPE;
+    hipError_t e = hipSuccess;
+    if (a.room) {
+        a.share = (uint32_t)std::max<uint64_t>(2u, groups * tiles / (4u * (uint64_t)ctx.compute_units));
+        a.splits = (uint32_t)((tiles + a.share - 1u) / a.share);
+        const size_t parts = a.splits == 1u ? 0 : (size_t)sequences * kv_heads * a.room * a.splits;
+        const size_t sums = (parts * sizeof(float2) + 255u) & ~(size_t)255u;
+        Workspace work(ctx.index, sums + parts * width * sizeof(float));
+        if (work.status) return work.status;
+        a.part_sums = (float2*)work.memory;
+        a.part = (float*)(work.memory + sums);
+        const uint32_t grid = (uint32_t)(groups * a.splits);
+        if (kind == TMH_CACHE_F32)
+            launch_few_of<TMH_CACHE_F32>(a, row_tiles, grid, ctx.stream);
+        else if (kind == TMH_CACHE_F16)
+            launch_few_of<TMH_CACHE_F16>(a, row_tiles, grid, ctx.stream);
+        else
+            launch_few_of<TMH_CACHE_BF16>(a, row_tiles, grid, ctx.stream);
+        e = hipGetLastError();
+        if (e == hipSuccess && a.splits > 1u) {
+            TMH_LAUNCH(k_attend_join, dim3(sequences * kv_heads * a.room), dim3(256), 0, ctx.stream, a);
+            e = hipGetLastError();
+        }
+    }
+    if (e == hipSuccess && (uint64_t)max_new * group > FEW_ROWS) {
+        AttendPaged b = a;
+        b.share = 1u << 30, b.splits = 1, b.room = 0;
+        const dim3 grid(tokens * heads);
+        if (kind == TMH_CACHE_F32)
+            TMH_LAUNCH(k_attend_row<TMH_CACHE_F32>, grid, dim3(256), 0, ctx.stream, b);
+        else if (kind == TMH_CACHE_F16)
+            TMH_LAUNCH(k_attend_row<TMH_CACHE_F16>, grid, dim3(256), 0, ctx.stream, b);
+        else
+            TMH_LAUNCH(k_attend_row<TMH_CACHE_BF16>, grid, dim3(256), 0, ctx.stream, b);
+        e = hipGetLastError();
+    }
     if (e == hipSuccess) note_launch(ctx.index, 1, true);
     return code(e);
 }

@@ -208,6 +208,7 @@ struct AttendPaged {
 constexpr uint32_t KEYS = 64;      // positions of a tile of keys
 constexpr uint32_t FEW_TILE = 16;  // query rows of a tile of few rows
 constexpr uint32_t FEW_ROWS = 32;  // the most query rows of a kv head that are few
+constexpr uint32_t ROW_TILE = 128;  // query rows of a tile of more
 
 // The tiles of keys that positions [lo, hi] see: `early` of the sinks, then
 // those from the window's first, `from`, on.
@@ -379,27 +380,6 @@ __device__ __forceinline__ void plain_rows(const AttendPaged& a, const Rows& w, 
     }
 }
 
-// One query row by one workgroup.
-template <uint32_t KIND>
-__global__ __launch_bounds__(256) void k_attend_row(AttendPaged a) {
-    const uint32_t t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-    Rows w;
-    w.s = sequence_of(a.p, t);
-    w.kh = a.group.divide(h);
-    if (w.s >= a.p.sequences || (int32_t)t < a.p.starts[0]) return;
-    const bool fits = read_sequence(a.p, w.s, w.sq);
-    const uint32_t i = t - w.sq.first;
-    if (!fits || i >= w.sq.count) {
-        if (threadIdx.x == 0 && h == 0) report(a.p.errors, (int32_t)w.s, (int32_t)a.p.sequences);
-        return;
-    }
-    if (w.sq.count * a.group.d <= FEW_ROWS) return;  // k_attend_few's
-    if (!w.set(a, i * a.group.d + h - w.kh * a.group.d, 1, 0)) return;
-    w.parts = 1, w.end = w.span.tiles;
-    const uint32_t first = 1;
-    plain_rows<KIND>(a, w, 0, &first);
-}
-
 // ------------------------------------------------------- on the matrix cores
 //
 // The matrix cores multiply 16-bit numbers exactly and add in f32, so f32
@@ -450,6 +430,12 @@ __device__ __forceinline__ void split_pair(Operand<Split<KIND>::PARTS>& o, int a
             v1 -= __uint_as_float(w1 & 0xffff0000u);
         }
     }
+}
+
+// Eight bytes of LDS a lane, turned: lanes 4r .. 4r + 3 of 16 name row r of four
+// rows of 16 numbers, and lane c gets column c of them.
+__device__ __forceinline__ uint64_t read_turned(const uint8_t* at) {
+    return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(const lds_byte*)at));
 }
 
 template <uint32_t KIND>
@@ -693,11 +679,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_
             } else {
                 // 4 rows of 16 columns a lane group, turned: 4 rows of a column a lane
                 const uint32_t row = group * 4u + col / 4u;
-                const uint32_t at = stage_at + buffer * F::STAGE + row * W * 2u +
-                                    F::swizzle(d * 2u + col % 4u / 2u, row) * 16u + col % 2u * 8u;
-                const uint64_t early = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at));
-                const uint64_t late = __builtin_bit_cast(
-                    uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(at + 16u * W * 2u)));
+                const uint8_t* at = from + row * W * 2u + F::swizzle(d * 2u + col % 4u / 2u, row) * 16u + col % 2u * 8u;
+                const uint64_t early = read_turned(at), late = read_turned(at + 16u * W * 2u);
                 o.part[0] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
             }
             out[d] = multiply_parts16<KIND>(o, weight, out[d]);
@@ -747,20 +730,337 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_
     if (again) plain_rows<KIND>(a, w, part, &again);
 }
 
+// --------------------------------------------------------------- more query rows
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <uint32_t KIND>
+__device__ __forceinline__ f32x16 multiply32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (KIND == TMH_CACHE_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <uint32_t KIND>
+__device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CACHE_PARTS>& a,
+                                                   const Operand<Split<KIND>::PARTS>& b, f32x16 c) {
+    constexpr int LAST = (int)Split<KIND>::PARTS - 1;
+#pragma unroll
+    for (int order = LAST; order >= 0; --order)
+#pragma unroll
+        for (int p = 0; p < (int)Split<KIND>::CACHE_PARTS; ++p)
+            if (order - p >= 0) c = multiply32<KIND>(a.part[p], b.part[order - p], c);
+    return c;
+}
+
+// Prompts and chunks: ROW_TILE query rows of a kv head, 32 a wave, against a
+// share of the keys, KT positions staged into LDS at a time for the four waves.
+// The products bound it, the softmax's vector operations next to them (about
+// ten a score; the products take 2 W cycles a 64 scores at two parts). So the
+// reference is not subtracted score by score: it is what the score's product
+// starts from. Scores are transposed as in k_attend_few; a lane then holds, of
+// each 32 keys, 4h..4h+3 of every eight for its half h of the wave, which are
+// the keys its second operand is given. F16 and BF16 tiles come by direct loads
+// into one of two buffers while the other is used; F32 ones are split in parts
+// on the way through registers, once for the four waves.
+template <uint32_t KIND, uint32_t W>
+struct Tile {
+    static constexpr bool F32 = KIND == TMH_CACHE_F32;
+    static constexpr uint32_t KT = W == 256u || (F32 && W == 128u) ? 32 : 64;
+    static constexpr uint32_t CHUNKS = W / 8u;  // of 8 columns: 16 bytes of LDS a part
+    static constexpr uint32_t PART = KT * W * 2u;
+    static constexpr uint32_t PARTS = Split<KIND>::CACHE_PARTS;
+    static constexpr uint32_t STAGE = 2u * PARTS * PART;  // keys, then values
+    static constexpr uint32_t LDS = F32 ? STAGE : 2u * STAGE;
+    static constexpr uint32_t LOADS = KT * CHUNKS / 256u;  // chunks a thread brings of keys, and of values
+    static __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t chunk, uint32_t row) {
+        return chunk ^ (row & (CHUNKS - 1u) & 7u);
+    }
+};
+
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
+    typedef Tile<KIND, W> T;
+    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ uint32_t redo[ROW_TILE / 32u];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
+    Rows w;
+    uint32_t b = blockIdx.x;
+    w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
+    const uint32_t part = b % a.splits;
+    uint32_t tile = b / a.splits;
+    // the sequence that row tile `tile` is in; a sequence's last rows, which
+    // see the most, first
+    bool found = false;
+    for (uint32_t i = 0; i < a.p.sequences; i += 64u) {
+        Sequence sq{};
+        uint32_t tiles = 0;
+        if (i + lane < a.p.sequences && read_sequence(a.p, i + lane, sq) && sq.count * a.group.d > FEW_ROWS)
+            tiles = (sq.count * a.group.d + ROW_TILE - 1u) / ROW_TILE;
+        uint32_t through = tiles;
+#pragma unroll
+        for (uint32_t d = 1; d < 64u; d <<= 1) {
+            const uint32_t o = __shfl_up(through, d, 64);
+            if (lane >= d) through += o;
+        }
+        const uint64_t past = __ballot(through > tile);
+        if (past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            w.s = i + (uint32_t)at;
+            w.sq.first = __builtin_amdgcn_readlane(sq.first, at);
+            w.sq.count = __builtin_amdgcn_readlane(sq.count, at);
+            w.sq.length = __builtin_amdgcn_readlane(sq.length, at);
+            tile = __builtin_amdgcn_readlane(through, at) - 1u - tile;
+            found = true;
+            break;
+        }
+        tile -= __builtin_amdgcn_readlane(through, 63);
+    }
+    if (!found || !w.set(a, tile * ROW_TILE, ROW_TILE, part)) return;
+    const uint32_t width = a.p.width;
+    const size_t row_bytes = (size_t)width * Split<KIND>::BYTES;
+
+    // this lane's query (rows past the tile's repeat its last), and the
+    // positions of the wave's
+    const uint32_t r = w.first + min(wave * 32u + col, w.count - 1u);
+    const uint32_t pos = w.position(a, r);
+    const bool idle = wave * 32u >= w.count;
+    const uint32_t lo = w.position(a, w.first + min(wave * 32u, w.count - 1u));
+    const uint32_t hi = w.position(a, w.first + min(wave * 32u + 31u, w.count - 1u));
+    Operand<NP> query[W / 16u];
+    float power = 1.0f, undo = 1.0f;
+    {
+        const float* q = a.q + (size_t)w.token(a, r) * a.ldq + w.head(a, r) * width;
+        float v[W / 16u][8];
+        float largest = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < W / 16u; ++k) {
+            const uint32_t c = k * 16u + half * 8u;
+            const Four* from = reinterpret_cast<const Four*>(q + (c < width ? c : 0u));
+            const Four lo4 = from[0], hi4 = from[1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[k][j] = c < width ? (j < 4 ? lo4.v[j & 3] : hi4.v[j & 3]) * a.scale : 0.0f;
+                largest = fmaxf(largest, fabsf(v[k][j]));
+            }
+        }
+        if (KIND == TMH_CACHE_F16) {
+            largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+            power = power_for(largest);
+            undo = 1.0f / power;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < W / 16u; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) split_pair<KIND>(query[k], j / 2, v[k][j] * power, v[k][j + 1] * power);
+    }
+
+    // step i: KT positions. A thread brings chunk at % CHUNKS of rows at /
+    // CHUNKS for at = threadIdx.x + 256 l (where a row is narrower than W its
+    // first columns stand in); the pages of the rows are looked up a step ahead.
+    constexpr uint32_t PER = KEYS / KT;
+    const uint32_t steps = PER * (w.end - w.begin);
+    const auto first_key = [&](uint32_t i) { return w.span.key(w.begin + i / PER) + i % PER * KT; };
+    uint32_t rows[T::LOADS];
+    const auto look_up = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t l = 0; l < T::LOADS; ++l)
+            rows[l] = w.cache_row_for(a, first_key(i) + (threadIdx.x + l * 256u) / T::CHUNKS);
+    };
+    const auto load_direct = [&](uint32_t buffer) {
+        const uint32_t to = lds_address(lds + buffer * T::STAGE + wave * 1024u);
+#pragma unroll
+        for (uint32_t l = 0; l < T::LOADS; ++l) {
+            const uint32_t at = threadIdx.x + l * 256u;
+            const uint32_t c = T::swizzle(at % T::CHUNKS, at / T::CHUNKS) * 16u;
+            const size_t from = (size_t)rows[l] * row_bytes + (c < row_bytes ? c : 0u);
+            lds_load16((const uint8_t*)a.keys + from, to + l * 4096u);
+            lds_load16((const uint8_t*)a.values + from, to + T::PART + l * 4096u);
+        }
+    };
+    f32x4 held[T::F32 ? T::LOADS : 1][2][2];
+    const auto load_held = [&]() {
+#pragma unroll
+        for (uint32_t l = 0; l < T::LOADS; ++l) {
+            const uint32_t c = (threadIdx.x + l * 256u) % T::CHUNKS * 32u;
+            const size_t from = (size_t)rows[l] * row_bytes + (c < row_bytes ? c : 0u);
+            held[l][0][0] = *(const f32x4*)((const uint8_t*)a.keys + from);
+            held[l][0][1] = *(const f32x4*)((const uint8_t*)a.keys + from + 16u);
+            held[l][1][0] = *(const f32x4*)((const uint8_t*)a.values + from);
+            held[l][1][1] = *(const f32x4*)((const uint8_t*)a.values + from + 16u);
+        }
+    };
+    const auto store_held = [&]() {
+#pragma unroll
+        for (uint32_t l = 0; l < T::LOADS; ++l) {
+            const uint32_t at = threadIdx.x + l * 256u, row = at / T::CHUNKS;
+#pragma unroll
+            for (uint32_t v = 0; v < 2u; ++v) {
+                Operand<NP> o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    split_pair<KIND>(o, j, held[l][v][j / 2][j % 2 * 2], held[l][v][j / 2][j % 2 * 2 + 1]);
+#pragma unroll
+                for (uint32_t p = 0; p < CP; ++p)
+                    *(u32x4*)(lds + (v * CP + p) * T::PART + row * W * 2u + T::swizzle(at % T::CHUNKS, row) * 16u) = o.part[p];
+            }
+        }
+    };
+
+    // Scores count from the reference: base is what their product starts from,
+    // (HEADROOM - reference) · power, limit HEADROOM + SLACK likewise, or -inf
+    // before the first score.
+    float base = 0.0f, limit = -INFINITY, total = 0.0f;
+    f32x16 out[W / 32u];
+#pragma unroll
+    for (uint32_t d = 0; d < W / 32u; ++d) out[d] = f32x16{} * 0.0f;
+    if (threadIdx.x < ROW_TILE / 32u) redo[threadIdx.x] = 0;
+    look_up(0);
+    if constexpr (T::F32)
+        load_held();
+    else
+        load_direct(0);
+    if (steps > 1u) look_up(1);
+    for (uint32_t i = 0; i < steps; ++i) {
+        const uint8_t* stage = lds;
+        if constexpr (T::F32) {
+            lds_sync();  // the last step's tile has been read
+            store_held();
+            lds_sync();
+            if (i + 1u < steps) load_held();
+        } else {
+            // this step's tile has landed, and every wave is past the last's
+            wait_vm_lds<0>();
+            lds_sync();
+            if (i + 1u < steps) load_direct((i + 1u) & 1u);
+            stage = lds + (i & 1u) * T::STAGE;
+        }
+        if (i + 2u < steps) look_up(i + 2u);
+        const uint32_t k0 = first_key(i);
+#pragma unroll
+        for (uint32_t g = 0; g < KT / 32u; ++g) {
+            const uint32_t kg = k0 + g * 32u;
+            // keys that none of the wave's rows sees
+            if (idle || kg > hi || (kg >= a.sinks && kg + 31u < window_start(a, lo))) continue;
+            f32x16 score;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) score[j] = base;
+#pragma unroll
+            for (uint32_t k = 0; k < W / 16u; ++k) {
+                Operand<CP> o;
+                const uint32_t row = g * 32u + col;
+#pragma unroll
+                for (uint32_t p = 0; p < CP; ++p)
+                    o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
+                score = multiply_parts32<KIND>(o, query[k], score);
+            }
+            const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
+            if (!whole) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j)
+                    if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
+            }
+            float best = score[0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
+            if (__any(best > limit)) {
+                best = fmaxf(best, __shfl_xor(best, 32, 64));
+                if (best > limit) {
+                    const float above = best - HEADROOM * power;
+                    const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-above * undo);
+                    base -= above;
+                    limit = (HEADROOM + SLACK) * power;
+                    total *= keep;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) score[j] -= above;
+#pragma unroll
+                    for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
+                }
+            }
+            Operand<NP> weight[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                if (KIND == TMH_CACHE_F16) score[j] *= undo, score[j + 1] *= undo;
+                const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
+                sum += e0;
+                sum += e1;
+                split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
+            }
+            total += sum;
+#pragma unroll
+            for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+                for (uint32_t c = 0; c < 2u; ++c) {
+                    // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
+                    Operand<CP> o;
+                    const uint32_t row = g * 32u + c * 16u + half * 4u + col % 16u / 4u;
+                    const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
+#pragma unroll
+                    for (uint32_t p = 0; p < CP; ++p) {
+                        const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
+                        const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
+                        const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
+                        o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
+                    }
+                    out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
+                }
+        }
+    }
+
+    total += __shfl_xor(total, 32, 64);
+    const uint32_t mine = wave * 32u + col;
+    if (mine < w.count) {
+        bool finite = total < INFINITY && (total > 0.0f || !w.sees_any(a, pos));
+        const float by = w.parts == 1u ? 1.0f / total : 1.0f;
+        const size_t at = w.place(a, r) + part;
+        float* to = w.parts == 1u ? a.dst + (size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width : a.part + at * width;
+        if (w.parts > 1u && half == 0) a.part_sums[at] = make_float2(limit == -INFINITY ? -INFINITY : -base * undo, total);
+#pragma unroll
+        for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e) {
+                const uint32_t c = d * 32u + e * 8u + half * 4u;
+                if (c >= width) continue;
+                Four o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    finite &= fabsf(out[d][e * 4u + j]) < INFINITY;
+                    o.v[j] = out[d][e * 4u + j] * by;
+                }
+                *reinterpret_cast<Four*>(to + c) = o;
+            }
+        if (!finite) atomicOr(&redo[mine / 32u], 1u << mine % 32u);
+    }
+    __syncthreads();
+    if (redo[0] | redo[1] | redo[2] | redo[3]) plain_rows<KIND>(a, w, part, redo);
+}
+
 // Joins the parts of a row: each brought to the highest reference, a wave
 // every fourth part.
 __global__ __launch_bounds__(256) void k_attend_join(AttendPaged a) {
     __shared__ float sums[4][256];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, width = a.p.width;
     Rows w;
-    uint32_t b = blockIdx.x;
-    const uint32_t r = b % a.room;
-    b /= a.room;
-    w.kh = b % a.p.kv_heads;
-    w.s = b / a.p.kv_heads;
-    if (!read_sequence(a.p, w.s, w.sq)) return;
-    const uint32_t rows = w.sq.count * a.group.d;
-    if (rows > FEW_ROWS || r >= rows || !w.set(a, r / FEW_TILE * FEW_TILE, FEW_TILE, 0) || w.parts == 1u) return;
+    uint32_t r;
+    if (a.room) {  // of few rows: by sequence, kv head and row
+        uint32_t b = blockIdx.x;
+        r = b % a.room;
+        b /= a.room;
+        w.kh = b % a.p.kv_heads;
+        w.s = b / a.p.kv_heads;
+        if (!read_sequence(a.p, w.s, w.sq)) return;
+    } else {  // by token and head
+        const uint32_t t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+        w.s = sequence_of(a.p, t);
+        w.kh = a.group.divide(h);
+        if (w.s >= a.p.sequences || !read_sequence(a.p, w.s, w.sq) || t < w.sq.first) return;
+        r = (t - w.sq.first) * a.group.d + h - w.kh * a.group.d;
+    }
+    const uint32_t rows = w.sq.count * a.group.d, size = a.room ? FEW_TILE : ROW_TILE;
+    if ((rows > FEW_ROWS) == (a.room != 0) || r >= rows || !w.set(a, r / size * size, size, 0) || w.parts == 1u) return;
     const size_t at = w.place(a, r);
     float top = -INFINITY;
     for (uint32_t z = lane; z < w.parts; z += 64u) top = fmaxf(top, a.part_sums[at + z].x);
@@ -808,11 +1108,58 @@ void launch_few_of(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipS
         launch_few<KIND, 256>(a, row_tiles, grid, stream);
 }
 
+template <uint32_t KIND, uint32_t W>
+void launch_tile(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
+    constexpr uint32_t lds = Tile<KIND, W>::LDS;
+    TMH_LAUNCH((k_attend_tile<KIND, W>), dim3(grid), dim3(256), lds, stream, a);
+}
+
+template <uint32_t KIND>
+void launch_tile_of(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
+    if (a.p.width <= 32u)
+        launch_tile<KIND, 32>(a, grid, stream);
+    else if (a.p.width <= 64u)
+        launch_tile<KIND, 64>(a, grid, stream);
+    else if (a.p.width <= 128u)
+        launch_tile<KIND, 128>(a, grid, stream);
+    else
+        launch_tile<KIND, 256>(a, grid, stream);
+}
+
 // Tiles of keys that a row tile of `tokens` new tokens sees, at most.
 uint64_t most_tiles(const AttendPaged& a, uint32_t tokens) {
     const uint64_t all = ((uint64_t)a.p.max_length + KEYS - 1u) / KEYS;
     if (a.window == 0u) return all;
     return std::min<uint64_t>(all, ((uint64_t)a.sinks + KEYS - 1u) / KEYS + ((uint64_t)a.window + tokens + KEYS) / KEYS + 1u);
+}
+
+// Shares of the keys for `groups` row tiles of at most `tiles` tiles of keys:
+// so that there are `wanted` workgroups, of at least `least` tiles each.
+void set_shares(AttendPaged& a, uint64_t groups, uint64_t tiles, uint64_t wanted, uint32_t least) {
+    a.share = (uint32_t)std::max<uint64_t>(least, groups * tiles / wanted);
+    a.splits = (uint32_t)std::max<uint64_t>(1u, (tiles + a.share - 1u) / a.share);
+}
+
+template <uint32_t KIND>
+hipError_t launch_attention_paged(const AttendPaged& few, uint32_t few_groups, uint32_t row_tiles,
+                                  const AttendPaged& more, uint32_t more_groups, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    if (more_groups) {
+        launch_tile_of<KIND>(more, more_groups * more.splits, stream);
+        e = hipGetLastError();
+        if (e == hipSuccess && more.splits > 1u) {
+            TMH_LAUNCH(k_attend_join, dim3(more.p.tokens * more.heads), dim3(256), 0, stream, more);
+            e = hipGetLastError();
+        }
+    }
+    if (e != hipSuccess) return e;
+    launch_few_of<KIND>(few, row_tiles, few_groups * few.splits, stream);
+    e = hipGetLastError();
+    if (e == hipSuccess && few.splits > 1u) {
+        TMH_LAUNCH(k_attend_join, dim3(few.p.sequences * few.p.kv_heads * few.room), dim3(256), 0, stream, few);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 int check_paged(uint32_t tokens, uint32_t kind, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t width,
@@ -888,48 +1235,38 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
                    tokens, max_new, max_length, pages, kv_heads, width, Divider(page_size), ctx.errors},
                   (const float*)q, ldq, heads, Divider(group), (const void*)keys, (const void*)values, window, sinks,
                   (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst, 0, 1, 0, nullptr, nullptr};
-    // few rows: shares of the keys such that four workgroups a compute unit
-    // have one each, of at least a step for each of their waves
-    a.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, (uint64_t)max_new * group);
-    const uint32_t row_tiles = (a.room + FEW_TILE - 1u) / FEW_TILE;
-    const uint64_t tiles = std::max<uint64_t>(1u, most_tiles(a, FEW_ROWS));
-    const uint64_t groups = (uint64_t)sequences * kv_heads * row_tiles;
-    if (groups > 0x7fffffffull) return TMH_ERROR_SHAPE;
-    hipError_t e = hipSuccess;
-    if (a.room) {
-        a.share = (uint32_t)std::max<uint64_t>(2u, groups * tiles / (4u * (uint64_t)ctx.compute_units));
-        a.splits = (uint32_t)((tiles + a.share - 1u) / a.share);
-        const size_t parts = a.splits == 1u ? 0 : (size_t)sequences * kv_heads * a.room * a.splits;
-        const size_t sums = (parts * sizeof(float2) + 255u) & ~(size_t)255u;
-        Workspace work(ctx.index, sums + parts * width * sizeof(float));
-        if (work.status) return work.status;
-        a.part_sums = (float2*)work.memory;
-        a.part = (float*)(work.memory + sums);
-        const uint32_t grid = (uint32_t)(groups * a.splits);
-        if (kind == TMH_CACHE_F32)
-            launch_few_of<TMH_CACHE_F32>(a, row_tiles, grid, ctx.stream);
-        else if (kind == TMH_CACHE_F16)
-            launch_few_of<TMH_CACHE_F16>(a, row_tiles, grid, ctx.stream);
-        else
-            launch_few_of<TMH_CACHE_BF16>(a, row_tiles, grid, ctx.stream);
-        e = hipGetLastError();
-        if (e == hipSuccess && a.splits > 1u) {
-            TMH_LAUNCH(k_attend_join, dim3(sequences * kv_heads * a.room), dim3(256), 0, ctx.stream, a);
-            e = hipGetLastError();
-        }
-    }
-    if (e == hipSuccess && (uint64_t)max_new * group > FEW_ROWS) {
-        AttendPaged b = a;
-        b.share = 1u << 30, b.splits = 1, b.room = 0;
-        const dim3 grid(tokens * heads);
-        if (kind == TMH_CACHE_F32)
-            TMH_LAUNCH(k_attend_row<TMH_CACHE_F32>, grid, dim3(256), 0, ctx.stream, b);
-        else if (kind == TMH_CACHE_F16)
-            TMH_LAUNCH(k_attend_row<TMH_CACHE_F16>, grid, dim3(256), 0, ctx.stream, b);
-        else
-            TMH_LAUNCH(k_attend_row<TMH_CACHE_BF16>, grid, dim3(256), 0, ctx.stream, b);
-        e = hipGetLastError();
-    }
+    // Few rows: shares of the keys such that four workgroups a compute unit
+    // have one each, of at least a step for each of their waves. More rows:
+    // two a compute unit, of at least eight tiles of keys.
+    AttendPaged few = a, more = a;
+    const uint64_t rows = std::max<uint64_t>(1u, (uint64_t)max_new * group);
+    few.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, rows);
+    const uint32_t row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
+    const uint64_t few_groups = (uint64_t)sequences * kv_heads * row_tiles;
+    const uint64_t few_tiles = most_tiles(a, FEW_ROWS);
+    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, 2u);
+    const bool has_more = rows > FEW_ROWS;
+    // row tiles of all sequences, at most
+    const uint64_t more_groups =
+        ((uint64_t)tokens * group / ROW_TILE + std::min<uint64_t>(sequences, (uint64_t)tokens * group / (FEW_ROWS + 1u))) * kv_heads;
+    if (has_more) set_shares(more, more_groups, most_tiles(a, ROW_TILE), 2u * ctx.compute_units, 8u);
+    if (few_groups * few.splits > 0x7fffffffull || more_groups * more.splits > 0x7fffffffull) return TMH_ERROR_SHAPE;
+    const size_t few_parts = few.splits > 1u ? (size_t)sequences * kv_heads * few.room * few.splits : 0;
+    const size_t more_parts = more.splits > 1u ? (size_t)tokens * heads * more.splits : 0;
+    const size_t sums = ((few_parts + more_parts) * sizeof(float2) + 255u) & ~(size_t)255u;
+    Workspace work(ctx.index, sums + (few_parts + more_parts) * width * sizeof(float));
+    if (work.status) return work.status;
+    few.part_sums = (float2*)work.memory;
+    few.part = (float*)(work.memory + sums);
+    more.part_sums = few.part_sums + few_parts;
+    more.part = few.part + few_parts * width;
+    hipError_t e;
+    if (kind == TMH_CACHE_F32)
+        e = launch_attention_paged<TMH_CACHE_F32>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
+    else if (kind == TMH_CACHE_F16)
+        e = launch_attention_paged<TMH_CACHE_F16>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
+    else
+        e = launch_attention_paged<TMH_CACHE_BF16>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
     if (e == hipSuccess) note_launch(ctx.index, 1, true);
     return code(e);
 }

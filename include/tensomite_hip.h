@@ -466,7 +466,7 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
  * not above 0 is tmh_argmax. temperature, top_k, top_p and min_p may each be 0
  * (no array): 1, all, 1 and 0. Sums and the weights are in 64 bits: the same
  * inputs give the same ids on every call. NaN is never chosen while another
- * candidate is there; n is at most 2^24. */
+ * candidate is there; n is at most 2^24, rows 65535. */
 int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t temperature, uint64_t top_k,
                uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids);
 

@@ -7,8 +7,8 @@
 // the token is the first whose running sum passes u·S. No row is sorted.
 // A histogram over y = (highest - x) · log2 e / t holds the count and the sum
 // of weights of each bin; the bin in which a count or a sum is reached is
-// looked up in it, and only few candidates are put in order: those through the
-// cut's bin where they are few, else those of that one bin.
+// looked up in it, and only few candidates are taken further: those through the
+// cut's bin where they fit the LDS, else those of that one bin.
 //
 // Weights are exp2 in f64, summed as integers of 2^-shift (shift = 62 less the
 // bits of n, at most 50: 45 at a vocabulary of 131071), so a sum is the same in
@@ -34,9 +34,9 @@ typedef unsigned long long u64;
 
 constexpr uint32_t THREADS = 1024, WAVES = THREADS / 64;
 constexpr uint32_t BINS = 2048;  // of y, two a thread
-constexpr uint32_t ZOOM = 1024;  // of keys, one a thread
-constexpr uint32_t LIST = 2048;  // candidates put in order at once, two a thread
-constexpr uint32_t PAIRS = 256;  // of which so many by comparing each with each
+constexpr uint32_t ZOOM = 1024;  // finer ones, of keys, one a thread
+constexpr uint32_t LIST = 4096;  // candidates held in LDS
+constexpr uint32_t FEW = 64;     // of which so many are put in order, one a lane
 
 // A chunk's highest value that is a number and its first index (or ~0), and
 // its lowest value but -inf.
@@ -47,6 +47,16 @@ struct Extent {
         low = fminf(low, o.low);
         if (o.index != ~0u && (index == ~0u || o.high > high || (o.high == high && o.index < index)))
             high = o.high, index = o.index;
+    }
+    __device__ __forceinline__ void take_wave() {
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) {
+            Extent o;
+            o.high = __shfl_xor(high, d, 64);
+            o.low = __shfl_xor(low, d, 64);
+            o.index = __shfl_xor(index, d, 64);
+            take(o);
+        }
     }
 };
 
@@ -84,8 +94,9 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 // 2^-y for y from 0 to 64: the exponent, and 2^f by its Taylor polynomial to
 // f^11 for f within half of 0 (off by less than 2^-46 of it).
 __device__ __forceinline__ double exp2_minus(double y) {
-    const double k = __builtin_rint(y);
-    const double f = (k - y) * 0.6931471805599453;
+    constexpr double ROUND = 6755399441055744.0;  // 1.5 · 2^52: what is added to it is rounded to integers
+    const double shifted = y + ROUND;
+    const double f = (shifted - ROUND - y) * 0.6931471805599453;
     double p = 1.0 / 39916800.0;
     p = __builtin_fma(p, f, 1.0 / 3628800.0);
     p = __builtin_fma(p, f, 1.0 / 362880.0);
@@ -98,7 +109,7 @@ __device__ __forceinline__ double exp2_minus(double y) {
     p = __builtin_fma(p, f, 0.5);
     p = __builtin_fma(p, f, 1.0);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, -(int)k);
+    return __builtin_bit_cast(double, __builtin_bit_cast(u64, p) - (__builtin_bit_cast(u64, shifted) << 52));
 }
 
 // A row's measure: its highest value, and y's scale, end and bins.
@@ -128,24 +139,27 @@ struct Measure {
     __device__ __forceinline__ u64 weight(double part) const {
         return (u64)__builtin_bit_cast(long long, part * one + 4503599627370496.0) & 0xfffffffffffffull;
     }
-    // The first key whose bin is `bin` or after it (keys not within cut are
-    // after all bins), by 64 keys a round.
-    __device__ __forceinline__ uint32_t first_key(uint32_t bin_from) const {
-        const uint32_t lane = threadIdx.x & 63u;
-        uint32_t low = key_of(highest), high = 0xff800000u;  // -inf's
+    // The first key whose bin is `from` or after it (keys not within cut are
+    // after all bins), by 64 keys a round: near where the bin should begin,
+    // else among all.
+    __device__ __forceinline__ bool past(uint32_t key, uint32_t from) const {
+        const float v = y(value_of(key));
+        return !within(v) || bin(v) >= from;
+    }
+    __device__ __forceinline__ uint32_t first_key(uint32_t from) const {
+        const uint32_t lane = threadIdx.x & 63u, first = key_of(highest), last = 0xff800000u;  // -inf's
+        const uint32_t guess = key_of(highest - (float)from / per_y / scale);
+        uint32_t low = max(first, guess - min(guess, 2048u)), high = min(last, guess + 2047u);
+        const bool near = low < high && (low == first || !past(low, from)) && (high == last || past(high, from));
+        if (!__all(near)) low = first, high = last;
         while (low < high) {
             const uint32_t step = (high - low - 1u) / 64u + 1u;
             const u64 at = (u64)low + (u64)step * lane;
-            bool past = at >= high;
-            if (!past) {
-                const float v = y(value_of((uint32_t)at));
-                past = !within(v) || bin(v) >= bin_from;
-            }
-            const uint64_t ones = __ballot(past);
-            const uint32_t first = ones ? (uint32_t)__ffsll((unsigned long long)ones) - 1u : 64u;
-            if (first == 0) return low;
-            high = (uint32_t)min((u64)high, (u64)low + (u64)step * first);
-            low = low + step * (first - 1u) + 1u;
+            const uint64_t ones = __ballot(at >= high || past((uint32_t)at, from));
+            const uint32_t n = ones ? (uint32_t)__ffsll((unsigned long long)ones) - 1u : 64u;
+            if (n == 0) return low;
+            high = (uint32_t)min((u64)high, (u64)low + (u64)step * n);
+            low = low + step * (n - 1u) + 1u;
         }
         return low;
     }
@@ -160,15 +174,27 @@ struct Found {
 
 struct Lds {
     u64 zoom_sums[ZOOM];
-    u64 list[LIST];     // key, then index
-    u64 sorted[LIST];
-    u64 through[LIST];  // sums through the sorted
+    u64 list[LIST];  // key, then index
+    u64 few[FEW];    // those of them the target is among
     uint32_t zoom_counts[ZOOM];
     u64 wave_sum[WAVES];
     uint32_t wave_count[WAVES];
     Found found;
-    uint32_t listed;
+    uint32_t listed, picked;
 };
+
+// v of the lane `CTRL` says, 0 where there is none or the row is not in MASK.
+template <int CTRL, int MASK>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, MASK, 0xF, true);
+}
+
+// One step of the wave's running sums.
+template <int CTRL, int MASK>
+__device__ __forceinline__ void scan_step(uint32_t& c, u64& s) {
+    c += dpp<CTRL, MASK>(c);
+    s += (u64)dpp<CTRL, MASK>((uint32_t)(s >> 32)) << 32 | dpp<CTRL, MASK>((uint32_t)s);
+}
 
 // Replaces count and sum by what the threads before this one hold of them;
 // all and total are everyone's.
@@ -176,18 +202,19 @@ __device__ __forceinline__ void scan(Lds& l, uint32_t& count, u64& sum, uint32_t
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     uint32_t c = count;
     u64 s = sum;
-#pragma unroll
-    for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint32_t oc = __shfl_up(c, d, 64);
-        const u64 os = __shfl_up(s, d, 64);
-        if (lane >= d) c += oc, s += os;
-    }
+    scan_step<0x111, 0xF>(c, s);  // 1, 2, 4 and 8 lanes back within each 16
+    scan_step<0x112, 0xF>(c, s);
+    scan_step<0x114, 0xF>(c, s);
+    scan_step<0x118, 0xF>(c, s);
+    scan_step<0x142, 0xA>(c, s);  // lane 15's to the next 16, lane 31's to the upper half
+    scan_step<0x143, 0xC>(c, s);
     __syncthreads();
     if (lane == 63u) l.wave_count[wave] = c, l.wave_sum[wave] = s;
     __syncthreads();
     uint32_t cb = 0;
     u64 sb = 0;
     all = 0, total = 0;
+#pragma unroll
     for (uint32_t w = 0; w < WAVES; ++w) {
         if (w == wave) cb = all, sb = total;
         all += l.wave_count[w], total += l.wave_sum[w];
@@ -230,89 +257,134 @@ struct Bins {
     }
 };
 
+// The bin of the finer histogram that the target is in, into l.found.
+__device__ __forceinline__ void find_zoomed(Lds& l, Target t, uint32_t count, u64 sum) {
+    Bins<1> bins;
+    uint32_t all;
+    u64 total;
+    bins.counts[0] = bins.count_before = l.zoom_counts[threadIdx.x];
+    bins.sums[0] = bins.sum_before = l.zoom_sums[threadIdx.x];
+    scan(l, bins.count_before, bins.sum_before, all, total);
+    bins.count_before += count, bins.sum_before += sum;
+    bins.find(l, t);
+}
+
+// Hands every value of row [from, to) with its index to `take`, over the
+// workgroup: four a load (of any alignment), AHEAD loads a thread in flight.
+struct alignas(4) Values {
+    float v[4];
+};
+
+template <uint32_t AHEAD, class TAKE>
+__device__ __forceinline__ void each_value(const float* row, uint32_t from, uint32_t to, TAKE take) {
+    constexpr uint32_t STEP = 4u * THREADS;
+    uint32_t j = from + 4u * threadIdx.x;
+    for (; j + (AHEAD - 1u) * STEP + 4u <= to; j += AHEAD * STEP) {
+        Values x[AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) x[i] = *reinterpret_cast<const Values*>(row + j + i * STEP);
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) take(x[i].v[k], j + i * STEP + k);
+    }
+    for (; j + 4u <= to; j += STEP) {
+        const Values x = *reinterpret_cast<const Values*>(row + j);
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; ++k) take(x.v[k], j + k);
+    }
+    for (; j < to; ++j) take(row[j], j);
+}
+
 // Lists the candidates with values from `low` to `high`: all of them into
 // l.listed, LIST at most into the list.
 __device__ __forceinline__ void list_values(Lds& l, const float* row, uint32_t n, float low, float high) {
     if (threadIdx.x == 0) l.listed = 0;
     __syncthreads();
-    const auto take = [&](float x, uint32_t j) {
+    each_value<8>(row, 0, n, [&](float x, uint32_t j) {
         if (x >= low && x <= high) {
             const uint32_t at = atomicAdd(&l.listed, 1u);
             if (at < LIST) l.list[at] = (u64)key_of(x) << 32 | j;
         }
-    };
-    constexpr uint32_t AHEAD = 8;
-    uint32_t j = threadIdx.x;
-    for (; j + (AHEAD - 1u) * THREADS < n; j += AHEAD * THREADS) {
-        float x[AHEAD];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) x[i] = row[j + i * THREADS];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) take(x[i], j + i * THREADS);
-    }
-    for (; j < n; j += THREADS) take(row[j], j);
+    });
     __syncthreads();
 }
 
-// Puts the list (at most LIST) in order, with the sums through each, `sum`
-// standing before the first.
-__device__ __forceinline__ void sort_list(Lds& l, const Measure& m, u64 sum) {
-    const uint32_t n = l.listed;
-    if (n > PAIRS) {  // a bitonic sort of the next power of two
-        uint32_t size = 2u * PAIRS;
-        while (size < n) size <<= 1;
-        for (uint32_t i = threadIdx.x; i < size; i += THREADS) l.sorted[i] = i < n ? l.list[i] : ~0ull;
-        for (uint32_t k = 2; k <= size; k <<= 1)
-            for (uint32_t d = k >> 1; d > 0; d >>= 1) {
-                __syncthreads();
-                if (threadIdx.x < size / 2u) {
-                    const uint32_t i = 2u * threadIdx.x - (threadIdx.x & (d - 1u));
-                    const u64 a = l.sorted[i], b = l.sorted[i + d];
-                    if ((a > b) == ((i & k) == 0)) l.sorted[i] = b, l.sorted[i + d] = a;
-                }
-            }
-    } else {
-        // four threads a candidate, each comparing it with a quarter of them
-        const uint32_t i = threadIdx.x >> 2;
-        const u64 mine = i < n ? l.list[i] : 0;
-        uint32_t c = 0;
-        if (i < n)
-            for (uint32_t j = threadIdx.x & 3u; j < n; j += 4u) c += l.list[j] < mine ? 1u : 0u;
-        c += __shfl_xor(c, 1, 64);
-        c += __shfl_xor(c, 2, 64);
-        if ((threadIdx.x & 3u) == 0 && i < n) l.sorted[c] = mine;
-    }
-    __syncthreads();
-    const uint32_t at = 2u * threadIdx.x;
-    u64 w[2];
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i)
-        w[i] = at + i < n ? m.weight(m.part(value_of((uint32_t)(l.sorted[at + i] >> 32)))) : 0;
-    uint32_t none = 0, all;
-    u64 before = w[0] + w[1], total;
-    scan(l, none, before, all, total);
-    l.through[at] = sum + before + w[0];
-    l.through[at + 1u] = sum + before + w[0] + w[1];
-    __syncthreads();
-}
+// Candidates one a lane of a wave, with what stands before each in their order.
+struct Few {
+    u64 mine, weight, sum;
+    uint32_t n, count;
 
-// The target among the sorted, `count` and `sum` standing before the first.
-__device__ __forceinline__ void find_sorted(Lds& l, Target t, uint32_t count, u64 sum) {
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t at = 2u * threadIdx.x + i;
-        if (at < l.listed) {
-            const u64 before = at ? l.through[at - 1u] : sum, through = l.through[at];
-            if (t.in(count + at, 1, before, through - before)) l.found.index = (uint32_t)l.sorted[at], l.found.sum = through;
+    __device__ __forceinline__ Few(const u64* from, uint32_t size, const Measure& m, uint32_t before, u64 sum_before)
+        : sum(sum_before), n(size), count(before) {
+        const uint32_t lane = threadIdx.x & 63u;
+        mine = lane < n ? from[lane] : ~0ull;
+        weight = lane < n ? m.weight(m.part(value_of((uint32_t)(mine >> 32)))) : 0;
+        for (uint32_t j = 0; j < n; ++j) {
+            const bool less = one(mine, j) < mine;
+            count += less ? 1u : 0u;
+            sum += less ? one(weight, j) : 0;
         }
+    }
+    static __device__ __forceinline__ u64 one(u64 v, uint32_t lane) {
+        return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), (int)lane) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane);
+    }
+    // The index of the candidate that the target is in, and the sum through it.
+    __device__ __forceinline__ uint32_t find(Target t, u64& through) const {
+        const uint64_t is = __ballot((threadIdx.x & 63u) < n && t.in(count, 1, sum, weight));
+        const uint32_t lane = is ? (uint32_t)__ffsll((unsigned long long)is) - 1u : 0u;
+        through = one(sum + weight, lane);
+        return (uint32_t)one(mine, lane);
+    }
+};
+
+// The candidate that the target is in among the listed (at most LIST) with keys
+// from low to high, which are as many and have as much before them as l.found
+// says, and the sum through it, into l.found: by histograms of ever fewer keys
+// and indices until a wave can put what is left in order.
+__device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, uint32_t key_low, uint32_t key_high) {
+    const uint32_t listed = l.listed;
+    u64 low = (u64)key_low << 32, high = (u64)key_high << 32 | 0xffffffffu, sum = l.found.sum_before;
+    uint32_t n = l.found.count, count = l.found.count_before;
+    while (n > FEW) {
+        uint32_t shift = 0;
+        while (((high - low) >> shift) >= ZOOM) ++shift;
+        __syncthreads();
+        l.zoom_counts[threadIdx.x] = 0, l.zoom_sums[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < listed; i += THREADS) {
+            const u64 c = l.list[i];
+            if (c >= low && c <= high) {
+                atomicAdd(&l.zoom_counts[(uint32_t)((c - low) >> shift)], 1u);
+                atomicAdd(&l.zoom_sums[(uint32_t)((c - low) >> shift)], m.weight(m.part(value_of((uint32_t)(c >> 32)))));
+            }
+        }
+        __syncthreads();
+        find_zoomed(l, t, count, sum);
+        count = l.found.count_before, sum = l.found.sum_before, n = l.found.count;
+        low += (u64)l.found.bin << shift;
+        high = min(high, low + ((u64)1 << shift) - 1u);
+    }
+    if (threadIdx.x == 0) l.picked = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < listed; i += THREADS) {
+        const u64 c = l.list[i];
+        if (c >= low && c <= high) l.few[atomicAdd(&l.picked, 1u)] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64u) {
+        const Few few(l.few, n, m, count, sum);
+        u64 through;
+        const uint32_t index = few.find(t, through);
+        if (threadIdx.x == 0) l.found.index = index, l.found.sum = through;
     }
     __syncthreads();
 }
 
 // The candidate that the target is in, and the sum through it, into l.found;
-// the target's bin is there.
-__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const float* row, uint32_t n, Target t) {
+// the target's bin is there. `listed`: the bin's candidates are.
+__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, bool listed) {
     uint32_t low = m.first_key(l.found.bin), high = m.first_key(l.found.bin + 1u) - 1u;
     // more than the list holds: histograms of ever fewer keys
     while (l.found.count > LIST && low < high) {
@@ -321,32 +393,23 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
         __syncthreads();
         l.zoom_counts[threadIdx.x] = 0, l.zoom_sums[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t j = threadIdx.x; j < n; j += THREADS) {
-            const float x = row[j];
+        each_value<4>(row, 0, n, [&](float x, uint32_t) {
             const uint32_t key = key_of(x);
             if (key >= low && key <= high) {
                 atomicAdd(&l.zoom_counts[(key - low) >> shift], 1u);
                 atomicAdd(&l.zoom_sums[(key - low) >> shift], m.weight(m.part(x)));
             }
-        }
+        });
         __syncthreads();
-        Bins<1> bins;
-        uint32_t all;
-        u64 total;
-        bins.counts[0] = bins.count_before = l.zoom_counts[threadIdx.x];
-        bins.sums[0] = bins.sum_before = l.zoom_sums[threadIdx.x];
-        scan(l, bins.count_before, bins.sum_before, all, total);
-        bins.count_before += l.found.count_before, bins.sum_before += l.found.sum_before;
-        bins.find(l, t);
+        find_zoomed(l, t, l.found.count_before, l.found.sum_before);
         low += l.found.bin << shift;
         high = min(high, low + (1u << shift) - 1u);
     }
     const uint32_t count = l.found.count_before;
     const u64 sum = l.found.sum_before;
     if (l.found.count <= LIST) {
-        list_values(l, row, n, value_of(high), value_of(low));
-        sort_list(l, m, sum);
-        find_sorted(l, t, count, sum);
+        if (!listed) list_values(l, row, n, value_of(high), value_of(low));
+        find_listed(l, m, t, low, high);
         return;
     }
     // one value more often than the list holds: by index
@@ -373,31 +436,14 @@ __global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
     const float* row = a.x + (size_t)blockIdx.y * a.ldx;
     const uint32_t from = blockIdx.x * a.chunk, to = min(from + a.chunk, a.n);
     Extent e{-INFINITY, INFINITY, ~0u};
-    const auto take = [&](float x, uint32_t j) {
+    each_value<4>(row, from, to, [&](float x, uint32_t j) {
         if (x == x && (e.index == ~0u || x > e.high)) e.high = x, e.index = j;
         if (x > -INFINITY) e.low = fminf(e.low, x);
-    };
-    constexpr uint32_t AHEAD = 8;
-    uint32_t j = from + threadIdx.x;
-    for (; j + (AHEAD - 1u) * THREADS < to; j += AHEAD * THREADS) {
-        float x[AHEAD];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) x[i] = row[j + i * THREADS];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) take(x[i], j + i * THREADS);
-    }
-    for (; j < to; j += THREADS) take(row[j], j);
+    });
     Histogram& h = a.rows[blockIdx.y];
     for (uint32_t b = blockIdx.x * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) h.least = 0;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        Extent o;
-        o.high = __shfl_xor(e.high, d, 64);
-        o.low = __shfl_xor(e.low, d, 64);
-        o.index = __shfl_xor(e.index, d, 64);
-        e.take(o);
-    }
+    e.take_wave();
     if (lane == 0) waves[wave] = e;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -408,8 +454,9 @@ __global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
 
 // A row's extent from its chunks', and whether it is to be sampled at all.
 __device__ __forceinline__ bool row_extent(const Sample& a, uint32_t r, float temperature, Extent& e) {
-    e = a.extents[(size_t)r * a.chunks];
-    for (uint32_t c = 1; c < a.chunks; ++c) e.take(a.extents[(size_t)r * a.chunks + c]);
+    e = Extent{-INFINITY, INFINITY, ~0u};
+    for (uint32_t c = threadIdx.x & 63u; c < a.chunks; c += 64u) e.take(a.extents[(size_t)r * a.chunks + c]);
+    e.take_wave();
     return temperature > 0.0f && e.high > -INFINITY;
 }
 
@@ -429,29 +476,19 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     for (uint32_t i = 0; i < BINS / THREADS; ++i) sums[threadIdx.x + i * THREADS] = 0, counts[threadIdx.x + i * THREADS] = 0;
     if (threadIdx.x == 0) least_sum = 0;
     __syncthreads();
+    const bool cut_least = !(least <= 0.0f);
     u64 kept = 0;
-    const auto take = [&](float x) {
+    each_value<4>(row, blockIdx.x * a.chunk, min(blockIdx.x * a.chunk + a.chunk, a.n), [&](float x, uint32_t) {
         const float y = m.y(x);
         if (m.within(y)) {
             const double part = m.part(x);
             const u64 weight = m.weight(part);
             atomicAdd(&counts[m.bin(y)], 1u);
             atomicAdd(&sums[m.bin(y)], weight);
-            if (part >= (double)least) kept += weight;
+            if (cut_least && part >= (double)least) kept += weight;
         }
-    };
-    const uint32_t from = blockIdx.x * a.chunk, to = min(from + a.chunk, a.n);
-    constexpr uint32_t AHEAD = 4;
-    uint32_t j = from + threadIdx.x;
-    for (; j + (AHEAD - 1u) * THREADS < to; j += AHEAD * THREADS) {
-        float x[AHEAD];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) x[i] = row[j + i * THREADS];
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) take(x[i]);
-    }
-    for (; j < to; j += THREADS) take(row[j]);
-    if (!(least <= 0.0f)) {
+    });
+    if (cut_least) {
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) kept += __shfl_xor(kept, d, 64);
         if ((threadIdx.x & 63u) == 0) atomicAdd(&least_sum, kept);
@@ -502,36 +539,48 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
     uint32_t all;
     u64 total;
     scan(l, bins.count_before, bins.sum_before, all, total);
-    // what is wanted of the histogram; where the candidates through a cut's
-    // bin fit the list, of them, in order, from then on
+    // the prefix that stays is the shortest of three: the sums through the
+    // k-th, through the first to reach p, and of weights of at least min_p
+    const bool cut_k = k > 0 && (uint32_t)k < all, cut_p = !(p >= 1.0f), cut_least = !(least <= 0.0f);
+    const Target kth{false, (u64)k - 1u};
+    const auto reach = [&](u64 of) {
+        const double sum = (double)p * (double)of;
+        return Target{true, sum > 0.0 ? (u64)__builtin_ceil(sum) - 1u : 0};
+    };
+    const auto choice = [&](u64 of) {
+        const double sum = (double)u * (double)of;
+        return Target{true, sum > 0.0 ? min((u64)sum, of - 1u) : sum == sum ? 0 : of - 1u};
+    };
+    const u64 first = (u64)1 << a.shift;  // the highest's weight: it always stays
     bool listed = false;
-    const auto find = [&](Target t, bool cut) {
-        if (!listed) {
-            bins.find(l, t);
-            if (!cut || l.found.count_before + l.found.count > LIST) {
-                find_in_bin(l, m, row, n, t);
+    if (cut_k || cut_p) {
+        bins.find(l, cut_k ? kth : reach(total));
+        if (l.found.count_before + l.found.count <= LIST) {
+            // the candidates through the cut's bin: of them from here on
+            listed = true;
+            list_values(l, row, n, value_of(m.first_key(l.found.bin + 1u) - 1u), m.highest);
+            if (l.listed <= FEW) {
+                if (threadIdx.x < 64u) {
+                    const Few few(l.list, l.listed, m, 0, 0);
+                    u64 through;
+                    if (cut_k) few.find(kth, total);
+                    if (cut_p) few.find(reach(total), through), total = min(total, through);
+                    if (cut_least) total = min(total, least_sum);
+                    const uint32_t index = few.find(choice(max(total, first)), through);
+                    if (threadIdx.x == 0) a.ids[r] = (int32_t)index;
+                }
                 return;
             }
-            list_values(l, row, n, value_of(m.first_key(l.found.bin + 1u) - 1u), m.highest);
-            sort_list(l, m, 0);
-            listed = true;
         }
-        find_sorted(l, t, 0, 0);
+    }
+    const auto find = [&](Target t) {
+        bins.find(l, t);
+        find_in_bin(l, m, row, n, t, listed);
     };
-    // the prefix that stays: the shortest of three
-    if (k > 0 && (uint32_t)k < all) {
-        find(Target{false, (u64)k - 1u}, true);
-        total = l.found.sum;
-    }
-    if (!(p >= 1.0f)) {
-        const double reach = (double)p * (double)total;
-        find(Target{true, reach > 0.0 ? (u64)__builtin_ceil(reach) - 1u : 0}, true);
-        total = min(total, l.found.sum);
-    }
-    if (!(least <= 0.0f)) total = min(total, least_sum);
-    total = max(total, (u64)1 << a.shift);
-    const double passes = (double)u * (double)total;
-    find(Target{true, passes > 0.0 ? min((u64)passes, total - 1u) : passes == passes ? 0 : total - 1u}, false);
+    if (cut_k) find(kth), total = l.found.sum;
+    if (cut_p) find(reach(total)), total = min(total, l.found.sum);
+    if (cut_least) total = min(total, least_sum);
+    find(choice(max(total, first)));
     if (threadIdx.x == 0) a.ids[r] = (int32_t)l.found.index;
 }
 

@@ -197,7 +197,7 @@ struct AttendPaged {
     uint32_t ld_dst;
     // Tiles of keys that one workgroup takes; where a row has more, its parts
     // (unscaled outputs; the reference score and the sum of weights) go to
-    // part and k_attend_join joins them. `splits` parts a row have room.
+    // part and the join kernels add them. `splits` parts a row have room.
     // The parts of few rows stand by sequence, kv head and row, `room` rows
     // each; those of other rows (room 0) by token and head.
     uint32_t share, splits, room;
@@ -466,11 +466,12 @@ __device__ __forceinline__ f32x4 multiply_parts16(const Operand<Split<KIND>::CAC
 constexpr float HEADROOM = 6.0f, SLACK = 8.0f;
 constexpr float NO_REFERENCE = -3.0e38f;
 
-// A power of two that brings the largest magnitude of a row of f16 parts to
-// 2^13 .. 2^14.
+// A power of two that brings the largest magnitude of a row to be split into
+// f16 parts to 2^13 .. 2^14; none where it is from 2^-3 to 2^13, at which the
+// parts' 2^-25 is 2^-22 of it already.
 __device__ __forceinline__ float power_for(float largest) {
     const int e = (int)(__float_as_uint(largest) >> 23) - 127;
-    if (largest == 0.0f || e > 127) return 1.0f;
+    if (largest == 0.0f || e > 127 || (e >= -3 && e < 13)) return 1.0f;
     return __uint_as_float((uint32_t)(min(13 - e, 126) + 127) << 23);
 }
 
@@ -757,9 +758,9 @@ __device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CA
 // Prompts and chunks: ROW_TILE query rows of a kv head, 32 a wave, against a
 // share of the keys, KT positions staged into LDS at a time for the four waves.
 // The products bound it, the softmax's vector operations next to them (about
-// ten a score; the products take 2 W cycles a 64 scores at two parts). So the
-// reference is not subtracted score by score: it is what the score's product
-// starts from. Scores are transposed as in k_attend_few; a lane then holds, of
+// eleven a score; the products take 2 W cycles a 64 scores at two parts), so the
+// products of the second 32 keys are out before the first's softmax begins.
+// Scores are transposed as in k_attend_few; a lane then holds, of
 // each 32 keys, 4h..4h+3 of every eight for its half h of the wave, which are
 // the keys its second operand is given. F16 and BF16 tiles come by direct loads
 // into one of two buffers while the other is used; F32 ones are split in parts
@@ -773,27 +774,18 @@ struct Tile {
     static constexpr uint32_t PARTS = Split<KIND>::CACHE_PARTS;
     static constexpr uint32_t STAGE = 2u * PARTS * PART;  // keys, then values
     static constexpr uint32_t LDS = F32 ? STAGE : 2u * STAGE;
+    static constexpr uint32_t AT_ONCE = W <= 64u ? 2 : 1;  // scores of so many times 32 keys before their softmax
     static constexpr uint32_t LOADS = KT * CHUNKS / 256u;  // chunks a thread brings of keys, and of values
     static __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t chunk, uint32_t row) {
         return chunk ^ (row & (CHUNKS - 1u) & 7u);
     }
 };
 
-template <uint32_t KIND, uint32_t W>
-__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
-    typedef Tile<KIND, W> T;
-    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ uint32_t redo[ROW_TILE / 32u];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
-    Rows w;
-    uint32_t b = blockIdx.x;
-    w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
-    const uint32_t part = b % a.splits;
-    uint32_t tile = b / a.splits;
-    // the sequence that row tile `tile` is in; a sequence's last rows, which
-    // see the most, first
-    bool found = false;
+// Sets w (its kv head is set) to part `part` of row tile `tile` of the sequences
+// with more than few rows; a sequence's last rows, which see the most, stand
+// first. Uniform over the wave, every lane active.
+__device__ __forceinline__ bool find_row_tile(const AttendPaged& a, uint32_t tile, uint32_t part, Rows& w) {
+    const uint32_t lane = threadIdx.x & 63u;
     for (uint32_t i = 0; i < a.p.sequences; i += 64u) {
         Sequence sq{};
         uint32_t tiles = 0;
@@ -812,13 +804,25 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
             w.sq.first = __builtin_amdgcn_readlane(sq.first, at);
             w.sq.count = __builtin_amdgcn_readlane(sq.count, at);
             w.sq.length = __builtin_amdgcn_readlane(sq.length, at);
-            tile = __builtin_amdgcn_readlane(through, at) - 1u - tile;
-            found = true;
-            break;
+            return w.set(a, (__builtin_amdgcn_readlane(through, at) - 1u - tile) * ROW_TILE, ROW_TILE, part);
         }
         tile -= __builtin_amdgcn_readlane(through, 63);
     }
-    if (!found || !w.set(a, tile * ROW_TILE, ROW_TILE, part)) return;
+    return false;
+}
+
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
+    typedef Tile<KIND, W> T;
+    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ uint32_t redo[ROW_TILE / 32u];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
+    Rows w;
+    uint32_t b = blockIdx.x;
+    w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
+    const uint32_t part = b % a.splits;
+    if (!find_row_tile(a, b / a.splits, part, w)) return;
     const uint32_t width = a.p.width;
     const size_t row_bytes = (size_t)width * Split<KIND>::BYTES;
 
@@ -909,10 +913,9 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         }
     };
 
-    // Scores count from the reference: base is what their product starts from,
-    // (HEADROOM - reference) · power, limit HEADROOM + SLACK likewise, or -inf
-    // before the first score.
-    float base = 0.0f, limit = -INFINITY, total = 0.0f;
+    // In units of the scores times power: zero is what weights count from (the
+    // reference less HEADROOM), limit the score that sets the reference anew.
+    float zero = 0.0f, limit = -INFINITY, total = 0.0f;
     f32x16 out[W / 32u];
 #pragma unroll
     for (uint32_t d = 0; d < W / 32u; ++d) out[d] = f32x16{} * 0.0f;
@@ -940,73 +943,78 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         if (i + 2u < steps) look_up(i + 2u);
         const uint32_t k0 = first_key(i);
 #pragma unroll
-        for (uint32_t g = 0; g < KT / 32u; ++g) {
-            const uint32_t kg = k0 + g * 32u;
+        for (uint32_t g0 = 0; g0 < KT / 32u; g0 += T::AT_ONCE) {
+            const uint32_t kg0 = k0 + g0 * 32u;
             // keys that none of the wave's rows sees
-            if (idle || kg > hi || (kg >= a.sinks && kg + 31u < window_start(a, lo))) continue;
-            f32x16 score;
+            if (idle || kg0 > hi || (kg0 >= a.sinks && kg0 + T::AT_ONCE * 32u <= window_start(a, lo))) continue;
+            f32x16 scores[T::AT_ONCE];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) score[j] = base;
+            for (uint32_t g = 0; g < T::AT_ONCE; ++g) {
+                scores[g] = f32x16{} * 0.0f;
 #pragma unroll
-            for (uint32_t k = 0; k < W / 16u; ++k) {
-                Operand<CP> o;
-                const uint32_t row = g * 32u + col;
-#pragma unroll
-                for (uint32_t p = 0; p < CP; ++p)
-                    o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
-                score = multiply_parts32<KIND>(o, query[k], score);
-            }
-            const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
-            if (!whole) {
-#pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j)
-                    if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
-            }
-            float best = score[0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
-            if (__any(best > limit)) {
-                best = fmaxf(best, __shfl_xor(best, 32, 64));
-                if (best > limit) {
-                    const float above = best - HEADROOM * power;
-                    const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-above * undo);
-                    base -= above;
-                    limit = (HEADROOM + SLACK) * power;
-                    total *= keep;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) score[j] -= above;
-#pragma unroll
-                    for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
-                }
-            }
-            Operand<NP> weight[2];
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-                if (KIND == TMH_CACHE_F16) score[j] *= undo, score[j + 1] *= undo;
-                const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
-                sum += e0;
-                sum += e1;
-                split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
-            }
-            total += sum;
-#pragma unroll
-            for (uint32_t d = 0; d < W / 32u; ++d)
-#pragma unroll
-                for (uint32_t c = 0; c < 2u; ++c) {
-                    // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
+                for (uint32_t k = 0; k < W / 16u; ++k) {
                     Operand<CP> o;
-                    const uint32_t row = g * 32u + c * 16u + half * 4u + col % 16u / 4u;
-                    const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
+                    const uint32_t row = (g0 + g) * 32u + col;
 #pragma unroll
-                    for (uint32_t p = 0; p < CP; ++p) {
-                        const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
-                        const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
-                        const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
-                        o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
-                    }
-                    out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
+                    for (uint32_t p = 0; p < CP; ++p)
+                        o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
+                    scores[g] = multiply_parts32<KIND>(o, query[k], scores[g]);
                 }
+            }
+#pragma unroll
+            for (uint32_t g = 0; g < T::AT_ONCE; ++g) {
+                f32x16& score = scores[g];
+                const uint32_t kg = kg0 + g * 32u;
+                const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
+                if (!whole) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j)
+                        if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
+                }
+                float best = score[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
+                if (__any(best > limit)) {
+                    best = fmaxf(best, __shfl_xor(best, 32, 64));
+                    if (best > limit) {
+                        const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((zero - best) * undo + HEADROOM);
+                        zero = best - HEADROOM * power;
+                        limit = best + SLACK * power;
+                        total *= keep;
+#pragma unroll
+                        for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
+                    }
+                }
+                Operand<NP> weight[2];
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    float e0 = score[j] - zero, e1 = score[j + 1] - zero;
+                    if (KIND == TMH_CACHE_F16) e0 *= undo, e1 *= undo;
+                    e0 = __builtin_amdgcn_exp2f(e0), e1 = __builtin_amdgcn_exp2f(e1);
+                    sum += e0;
+                    sum += e1;
+                    split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
+                }
+                total += sum;
+#pragma unroll
+                for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+                    for (uint32_t c = 0; c < 2u; ++c) {
+                        // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
+                        Operand<CP> o;
+                        const uint32_t row = (g0 + g) * 32u + c * 16u + half * 4u + col % 16u / 4u;
+                        const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
+#pragma unroll
+                        for (uint32_t p = 0; p < CP; ++p) {
+                            const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
+                            const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
+                            const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
+                            o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
+                        }
+                        out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
+                    }
+            }
         }
     }
 
@@ -1017,7 +1025,7 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         const float by = w.parts == 1u ? 1.0f / total : 1.0f;
         const size_t at = w.place(a, r) + part;
         float* to = w.parts == 1u ? a.dst + (size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width : a.part + at * width;
-        if (w.parts > 1u && half == 0) a.part_sums[at] = make_float2(limit == -INFINITY ? -INFINITY : -base * undo, total);
+        if (w.parts > 1u && half == 0) a.part_sums[at] = make_float2(limit == -INFINITY ? -INFINITY : zero * undo, total);
 #pragma unroll
         for (uint32_t d = 0; d < W / 32u; ++d)
 #pragma unroll
@@ -1038,56 +1046,89 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
     if (redo[0] | redo[1] | redo[2] | redo[3]) plain_rows<KIND>(a, w, part, redo);
 }
 
-// Joins the parts of a row: each brought to the highest reference, a wave
-// every fourth part.
-__global__ __launch_bounds__(256) void k_attend_join(AttendPaged a) {
-    __shared__ float sums[4][256];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, width = a.p.width;
-    Rows w;
-    uint32_t r;
-    if (a.room) {  // of few rows: by sequence, kv head and row
-        uint32_t b = blockIdx.x;
-        r = b % a.room;
-        b /= a.room;
-        w.kh = b % a.p.kv_heads;
-        w.s = b / a.p.kv_heads;
-        if (!read_sequence(a.p, w.s, w.sq)) return;
-    } else {  // by token and head
-        const uint32_t t = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-        w.s = sequence_of(a.p, t);
-        w.kh = a.group.divide(h);
-        if (w.s >= a.p.sequences || !read_sequence(a.p, w.s, w.sq) || t < w.sq.first) return;
-        r = (t - w.sq.first) * a.group.d + h - w.kh * a.group.d;
-    }
-    const uint32_t rows = w.sq.count * a.group.d, size = a.room ? FEW_TILE : ROW_TILE;
-    if ((rows > FEW_ROWS) == (a.room != 0) || r >= rows || !w.set(a, r / size * size, size, 0) || w.parts == 1u) return;
+// Joins the parts of row r, by a wave: each part brought to the highest reference
+// and added. The parts wait in L2 or memory, so latency bounds it: a load takes
+// 64 / (width / 4) parts, and eight loads go out before the first is used.
+__device__ __forceinline__ void join_row(const AttendPaged& a, const Rows& w, uint32_t r, f32x4* lanes) {
+    const uint32_t lane = threadIdx.x & 63u, width = a.p.width, quads = width / 4u;
     const size_t at = w.place(a, r);
-    float top = -INFINITY;
-    for (uint32_t z = lane; z < w.parts; z += 64u) top = fmaxf(top, a.part_sums[at + z].x);
+    // lane: columns 4 (lane % quads) .. + 3 of part lane / quads of each load
+    constexpr uint32_t AHEAD = 8;
+    const uint32_t each = 64u / quads, mine = lane / quads, col = lane % quads * 4u;
+    float top = -INFINITY, total = 0.0f;
+    f32x4 out{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t z0 = 0; z0 < w.parts; z0 += AHEAD * each) {
+        Four part[AHEAD];
+        float2 sums[AHEAD];
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f;
-    for (uint32_t z = lane; z < w.parts; z += 64u) {
-        const float2 one = a.part_sums[at + z];
-        total += one.y * __builtin_amdgcn_exp2f(one.x - ref);
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t z = z0 + i * each + mine;
+            if (z0 + i * each >= w.parts) break;
+            const size_t from = at + (mine < each && z < w.parts ? z : z0);
+            part[i] = *reinterpret_cast<const Four*>(a.part + from * width + col);
+            sums[i] = a.part_sums[from];
+            if (mine >= each || z >= w.parts) sums[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float best = top;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            if (z0 + i * each < w.parts) best = fmaxf(best, sums[i].x);
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) best = fmaxf(best, __shfl_xor(best, d, 64));
+        const float ref = best == -INFINITY ? 0.0f : best;
+        const float keep = __builtin_amdgcn_exp2f(top - ref);
+        top = best;
+        total *= keep;
+        out *= keep;
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t z = z0 + i * each + mine;
+            if (mine >= each || z >= w.parts) continue;
+            const float by = __builtin_amdgcn_exp2f(sums[i].x - ref);
+            total += sums[i].y * by;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[j] += part[i].v[j] * by;
+        }
     }
+    // the lanes of a column, and one column's of every part's sum
+    lanes[lane] = out;
+    if (lane % quads != 0) total = 0.0f;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, 64);
-    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t z = wave; z < w.parts; z += 4u) {
-        const float keep = __builtin_amdgcn_exp2f(a.part_sums[at + z].x - ref);
+    if (lane < quads) {
+        for (uint32_t e = 1; e < each; ++e) out += lanes[lane + e * quads];
+        Four o;
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i)
-            if (lane + i * 64u < width) out[i] += a.part[(at + z) * width + lane + i * 64u] * keep;
+        for (int j = 0; j < 4; ++j) o.v[j] = out[j] / total;
+        *reinterpret_cast<Four*>(a.dst + (size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width + col) = o;
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) sums[wave][lane + i * 64u] = out[i];
-    __syncthreads();
-    const uint32_t c = threadIdx.x;
-    if (c < width)
-        a.dst[(size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width + c] =
-            (sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c]) / total;
+}
+
+// Joins few rows, a wave a row, by sequence, kv head and row.
+__global__ __launch_bounds__(256) void k_attend_join_few(AttendPaged a, uint32_t count) {
+    __shared__ f32x4 lanes[4][64];
+    uint32_t b = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (b >= count) return;
+    Rows w;
+    const uint32_t r = b % a.room;
+    b /= a.room;
+    w.kh = b % a.p.kv_heads;
+    w.s = b / a.p.kv_heads;
+    if (!read_sequence(a.p, w.s, w.sq)) return;
+    const uint32_t rows = w.sq.count * a.group.d;
+    if (rows > FEW_ROWS || r >= rows || !w.set(a, r / FEW_TILE * FEW_TILE, FEW_TILE, 0) || w.parts == 1u) return;
+    join_row(a, w, r, lanes[threadIdx.x >> 6]);
+}
+
+// Joins a quarter of a row tile, eight rows a wave.
+__global__ __launch_bounds__(256) void k_attend_join_tile(AttendPaged a) {
+    __shared__ f32x4 lanes[4][64];
+    Rows w;
+    w.kh = blockIdx.x % a.p.kv_heads;
+    if (!find_row_tile(a, blockIdx.x / a.p.kv_heads, 0, w) || w.parts == 1u) return;
+    const uint32_t from = blockIdx.y * (ROW_TILE / 4u) + (threadIdx.x >> 6) * (ROW_TILE / 16u);
+    for (uint32_t i = from; i < min(from + ROW_TILE / 16u, w.count); ++i)
+        join_row(a, w, w.first + i, lanes[threadIdx.x >> 6]);
 }
 
 template <uint32_t KIND, uint32_t W>
@@ -1148,7 +1189,7 @@ hipError_t launch_attention_paged(const AttendPaged& few, uint32_t few_groups, u
         launch_tile_of<KIND>(more, more_groups * more.splits, stream);
         e = hipGetLastError();
         if (e == hipSuccess && more.splits > 1u) {
-            TMH_LAUNCH(k_attend_join, dim3(more.p.tokens * more.heads), dim3(256), 0, stream, more);
+            TMH_LAUNCH(k_attend_join_tile, dim3(more_groups, 4), dim3(256), 0, stream, more);
             e = hipGetLastError();
         }
     }
@@ -1156,7 +1197,8 @@ hipError_t launch_attention_paged(const AttendPaged& few, uint32_t few_groups, u
     launch_few_of<KIND>(few, row_tiles, few_groups * few.splits, stream);
     e = hipGetLastError();
     if (e == hipSuccess && few.splits > 1u) {
-        TMH_LAUNCH(k_attend_join, dim3(few.p.sequences * few.p.kv_heads * few.room), dim3(256), 0, stream, few);
+        const uint32_t rows = few.p.sequences * few.p.kv_heads * few.room;
+        TMH_LAUNCH(k_attend_join_few, dim3((rows + 3u) / 4u), dim3(256), 0, stream, few, rows);
         e = hipGetLastError();
     }
     return e;

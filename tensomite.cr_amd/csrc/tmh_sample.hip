@@ -70,7 +70,7 @@ struct Histogram {
 struct Sample {
     const float* x;
     uint32_t ldx, n, shift;
-    uint32_t chunk, chunks;  // values of a chunk, chunks of a row
+    uint32_t chunk, chunks, count;  // values of a chunk, chunks of a row, rows
     const float* temperature;
     const int32_t* top_k;
     const float* top_p;
@@ -115,7 +115,7 @@ __device__ __forceinline__ double exp2_minus(double y) {
 // A row's measure: its highest value, and y's scale, end and bins.
 struct Measure {
     float highest, scale, cut, per_y;
-    double exact, one;  // the scale in f64; 2^shift
+    double exact, bin_y, one;  // the scale in f64; a bin's y; 2^shift
 
     __device__ __forceinline__ Measure(const Extent& e, float temperature, uint32_t shift) {
         highest = e.high;
@@ -125,19 +125,35 @@ struct Measure {
         one = (double)((u64)1 << shift);
         const float range = fminf((e.high - e.low) * scale, cut);
         per_y = range > 0.0f ? fminf((float)BINS / range, 1e30f) : 0.0f;
+        bin_y = range > 0.0f ? 1.0 / (double)per_y : 0.0;
     }
     // y in f32 falls as x rises, so bins stand in the candidates' order, and
     // y above cut is a weight of none. NaN and -inf are not within it.
     __device__ __forceinline__ float y(float x) const { return x == highest ? 0.0f : (highest - x) * scale; }
     __device__ __forceinline__ bool within(float y) const { return y <= cut; }
     __device__ __forceinline__ uint32_t bin(float y) const { return min((uint32_t)(y * per_y), BINS - 1u); }
-    __device__ __forceinline__ double part(float x) const {
-        return x == highest ? 1.0 : exp2_minus(((double)highest - (double)x) * exact);
+    // A weight of 2^shift for the highest is that at the bin's beginning times
+    // 2^-rest, the rest of y (at most 52 / BINS) by its Taylor polynomial to
+    // the fifth power, off by less than 2^-44 of it.
+    __device__ __forceinline__ double begin(uint32_t bin) const { return exp2_minus((double)bin * bin_y) * one; }
+    __device__ __forceinline__ double scaled(float x, uint32_t bin, double begin) const {
+        const double y = x == highest ? 0.0 : ((double)highest - (double)x) * exact;
+        const double rest = __builtin_fma((double)bin, -bin_y, y);
+        double p = -0.0013333558146428443;  // (-ln 2)^k / k!
+        p = __builtin_fma(p, rest, 0.009618129107628477);
+        p = __builtin_fma(p, rest, -0.05550410866482158);
+        p = __builtin_fma(p, rest, 0.2402265069591007);
+        p = __builtin_fma(p, rest, -0.6931471805599453);
+        p = __builtin_fma(p, rest, 1.0);
+        return begin * p;
     }
-    // to the nearest integer of 2^-shift, at most 2^50, in the low bits of a
-    // number of 2^52
-    __device__ __forceinline__ u64 weight(double part) const {
-        return (u64)__builtin_bit_cast(long long, part * one + 4503599627370496.0) & 0xfffffffffffffull;
+    // to the nearest integer (at most 2^50), in the low bits of a number of 2^52
+    static __device__ __forceinline__ u64 whole(double scaled) {
+        return (u64)__builtin_bit_cast(long long, scaled + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 weight(float x) const {
+        const uint32_t b = bin(y(x));
+        return whole(scaled(x, b, begin(b)));
     }
     // The first key whose bin is `from` or after it (keys not within cut are
     // after all bins), by 64 keys a round: near where the bin should begin,
@@ -296,8 +312,8 @@ __device__ __forceinline__ void each_value(const float* row, uint32_t from, uint
     for (; j < to; ++j) take(row[j], j);
 }
 
-// Lists the candidates with values from `low` to `high`: all of them into
-// l.listed, LIST at most into the list.
+// Lists the candidates with values from `low` to `high`: all of them counted in
+// l.listed, LIST at most in the list.
 __device__ __forceinline__ void list_values(Lds& l, const float* row, uint32_t n, float low, float high) {
     if (threadIdx.x == 0) l.listed = 0;
     __syncthreads();
@@ -319,7 +335,7 @@ struct Few {
         : sum(sum_before), n(size), count(before) {
         const uint32_t lane = threadIdx.x & 63u;
         mine = lane < n ? from[lane] : ~0ull;
-        weight = lane < n ? m.weight(m.part(value_of((uint32_t)(mine >> 32)))) : 0;
+        weight = lane < n ? m.weight(value_of((uint32_t)(mine >> 32))) : 0;
         for (uint32_t j = 0; j < n; ++j) {
             const bool less = one(mine, j) < mine;
             count += less ? 1u : 0u;
@@ -357,7 +373,7 @@ __device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, 
             const u64 c = l.list[i];
             if (c >= low && c <= high) {
                 atomicAdd(&l.zoom_counts[(uint32_t)((c - low) >> shift)], 1u);
-                atomicAdd(&l.zoom_sums[(uint32_t)((c - low) >> shift)], m.weight(m.part(value_of((uint32_t)(c >> 32)))));
+                atomicAdd(&l.zoom_sums[(uint32_t)((c - low) >> shift)], m.weight(value_of((uint32_t)(c >> 32))));
             }
         }
         __syncthreads();
@@ -397,7 +413,7 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
             const uint32_t key = key_of(x);
             if (key >= low && key <= high) {
                 atomicAdd(&l.zoom_counts[(key - low) >> shift], 1u);
-                atomicAdd(&l.zoom_sums[(key - low) >> shift], m.weight(m.part(x)));
+                atomicAdd(&l.zoom_sums[(key - low) >> shift], m.weight(x));
             }
         });
         __syncthreads();
@@ -413,7 +429,7 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
         return;
     }
     // one value more often than the list holds: by index
-    const u64 weight = m.weight(m.part(value_of(low)));
+    const u64 weight = m.weight(value_of(low));
     const u64 place = t.by_sum ? (t.target - sum) / weight : t.target - count;
     uint32_t before = 0;
     for (uint32_t base = 0; base < n; base += THREADS) {
@@ -428,27 +444,31 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
     __syncthreads();
 }
 
-// The highest and lowest values of chunk blockIdx.x of row blockIdx.y, whose
-// share of the row's histogram it clears.
+// The highest and lowest values of chunk blockIdx.y of row blockIdx.x, whose
+// share of the row's histogram it clears. Rows stand first in the grid, up to
+// a multiple of eight: a row's chunks then meet on one XCD, whose L2 holds the
+// row for the later launches.
 __global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
     __shared__ Extent waves[WAVES];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const float* row = a.x + (size_t)blockIdx.y * a.ldx;
-    const uint32_t from = blockIdx.x * a.chunk, to = min(from + a.chunk, a.n);
+    const uint32_t r = blockIdx.x, chunk = blockIdx.y;
+    if (r >= a.count) return;
+    const float* row = a.x + (size_t)r * a.ldx;
+    const uint32_t from = chunk * a.chunk, to = min(from + a.chunk, a.n);
     Extent e{-INFINITY, INFINITY, ~0u};
     each_value<4>(row, from, to, [&](float x, uint32_t j) {
         if (x == x && (e.index == ~0u || x > e.high)) e.high = x, e.index = j;
         if (x > -INFINITY) e.low = fminf(e.low, x);
     });
-    Histogram& h = a.rows[blockIdx.y];
-    for (uint32_t b = blockIdx.x * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) h.least = 0;
+    Histogram& h = a.rows[r];
+    for (uint32_t b = chunk * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
+    if (chunk == 0 && threadIdx.x == 0) h.least = 0;
     e.take_wave();
     if (lane == 0) waves[wave] = e;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (uint32_t w = 1; w < WAVES; ++w) e.take(waves[w]);
-        a.extents[(size_t)blockIdx.y * a.chunks + blockIdx.x] = e;
+        a.extents[(size_t)r * a.chunks + chunk] = e;
     }
 }
 
@@ -460,32 +480,38 @@ __device__ __forceinline__ bool row_extent(const Sample& a, uint32_t r, float te
     return temperature > 0.0f && e.high > -INFINITY;
 }
 
-// The histogram of chunk blockIdx.x of row blockIdx.y, added to the row's.
+// The histogram of chunk blockIdx.y of row blockIdx.x, added to the row's.
 __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     __shared__ u64 sums[BINS];
+    __shared__ double begins[BINS];
     __shared__ uint32_t counts[BINS];
     __shared__ u64 least_sum;
-    const uint32_t r = blockIdx.y;
+    const uint32_t r = blockIdx.x;
+    if (r >= a.count) return;
     const float* row = a.x + (size_t)r * a.ldx;
     const float temperature = a.temperature ? a.temperature[r] : 1.0f;
     Extent e;
     if (!row_extent(a, r, temperature, e)) return;
     const Measure m(e, temperature, a.shift);
-    const float least = a.min_p ? a.min_p[r] : 0.0f;
+    const double least = a.min_p ? (double)a.min_p[r] * m.one : 0.0;
 #pragma unroll
-    for (uint32_t i = 0; i < BINS / THREADS; ++i) sums[threadIdx.x + i * THREADS] = 0, counts[threadIdx.x + i * THREADS] = 0;
+    for (uint32_t i = 0; i < BINS / THREADS; ++i) {
+        const uint32_t b = threadIdx.x + i * THREADS;
+        sums[b] = 0, counts[b] = 0, begins[b] = m.begin(b);
+    }
     if (threadIdx.x == 0) least_sum = 0;
     __syncthreads();
-    const bool cut_least = !(least <= 0.0f);
+    const bool cut_least = !(least <= 0.0);
     u64 kept = 0;
-    each_value<4>(row, blockIdx.x * a.chunk, min(blockIdx.x * a.chunk + a.chunk, a.n), [&](float x, uint32_t) {
+    each_value<4>(row, blockIdx.y * a.chunk, min(blockIdx.y * a.chunk + a.chunk, a.n), [&](float x, uint32_t) {
         const float y = m.y(x);
         if (m.within(y)) {
-            const double part = m.part(x);
-            const u64 weight = m.weight(part);
-            atomicAdd(&counts[m.bin(y)], 1u);
-            atomicAdd(&sums[m.bin(y)], weight);
-            if (cut_least && part >= (double)least) kept += weight;
+            const uint32_t bin = m.bin(y);
+            const double scaled = m.scaled(x, bin, begins[bin]);
+            const u64 weight = m.whole(scaled);
+            atomicAdd(&counts[bin], 1u);
+            atomicAdd(&sums[bin], weight);
+            if (cut_least && scaled >= least) kept += weight;
         }
     });
     if (cut_least) {
@@ -611,10 +637,10 @@ int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t tem
     const size_t extents = ((size_t)rows * chunks * sizeof(Extent) + 255u) & ~(size_t)255u;
     Workspace work(ctx.index, extents + (size_t)rows * sizeof(Histogram));
     if (work.status) return work.status;
-    Sample a{(const float*)x, ldx, n, std::min(62u - bits, 50u), chunk, (n + chunk - 1u) / chunk,
+    Sample a{(const float*)x, ldx, n, std::min(62u - bits, 50u), chunk, (n + chunk - 1u) / chunk, rows,
              (const float*)temperature, (const int32_t*)top_k, (const float*)top_p, (const float*)min_p,
              (const float*)u, (int32_t*)ids, (Extent*)work.memory, (Histogram*)(work.memory + extents)};
-    const dim3 grid(a.chunks, rows);
+    const dim3 grid((rows + 7u) / 8u * 8u, a.chunks);
     TMH_LAUNCH(k_sample_extent, grid, dim3(THREADS), 0, ctx.stream, a);
     TMH_LAUNCH(k_sample_histogram, grid, dim3(THREADS), 0, ctx.stream, a);
     TMH_LAUNCH(k_sample, dim3(rows), dim3(THREADS), sizeof(Lds), ctx.stream, a);

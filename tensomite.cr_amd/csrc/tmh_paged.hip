@@ -201,6 +201,8 @@ struct AttendPaged {
     // The parts of few rows stand by sequence, kv head and row, `room` rows
     // each; those of other rows (room 0) by token and head.
     uint32_t share, splits, room;
+    uint32_t row_tile;  // query rows of a tile of more than few
+    uint32_t alone;     // k_attend_tile takes sequences of few rows too
     float* part;
     float2* part_sums;
 };
@@ -208,7 +210,6 @@ struct AttendPaged {
 constexpr uint32_t KEYS = 64;      // positions of a tile of keys
 constexpr uint32_t FEW_TILE = 16;  // query rows of a tile of few rows
 constexpr uint32_t FEW_ROWS = 32;  // the most query rows of a kv head that are few
-constexpr uint32_t ROW_TILE = 128;  // query rows of a tile of more
 
 // The tiles of keys that positions [lo, hi] see: `early` of the sinks, then
 // those from the window's first, `from`, on.
@@ -755,7 +756,7 @@ __device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CA
     return c;
 }
 
-// Prompts and chunks: ROW_TILE query rows of a kv head, 32 a wave, against a
+// Prompts and chunks: 128 / KS query rows of a kv head, 32 a wave, against a
 // share of the keys, KT positions staged into LDS at a time for the four waves.
 // The products bound it, the softmax's vector operations next to them (about
 // eleven a score; the products take 2 W cycles a 64 scores at two parts), so the
@@ -765,8 +766,9 @@ __device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CA
 // the keys its second operand is given. F16 and BF16 tiles come by direct loads
 // into one of two buffers while the other is used; F32 ones are split in parts
 // on the way through registers, once for the four waves.
-template <uint32_t KIND, uint32_t W>
+template <uint32_t KIND, uint32_t W, uint32_t KS>
 struct Tile {
+    static constexpr uint32_t ROWS = 128u / KS;  // query rows of a workgroup
     static constexpr bool F32 = KIND == TMH_CACHE_F32;
     static constexpr uint32_t KT = W == 256u || (F32 && W == 128u) ? 32 : 64;
     static constexpr uint32_t CHUNKS = W / 8u;  // of 8 columns: 16 bytes of LDS a part
@@ -774,7 +776,7 @@ struct Tile {
     static constexpr uint32_t PARTS = Split<KIND>::CACHE_PARTS;
     static constexpr uint32_t STAGE = 2u * PARTS * PART;  // keys, then values
     static constexpr uint32_t LDS = F32 ? STAGE : 2u * STAGE;
-    static constexpr uint32_t AT_ONCE = W <= 64u ? 2 : 1;  // scores of so many times 32 keys before their softmax
+    static constexpr uint32_t AT_ONCE = W <= 64u && KS == 1u ? 2 : 1;  // scores of so many times 32 keys before their softmax
     static constexpr uint32_t LOADS = KT * CHUNKS / 256u;  // chunks a thread brings of keys, and of values
     static __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t chunk, uint32_t row) {
         return chunk ^ (row & (CHUNKS - 1u) & 7u);
@@ -789,8 +791,8 @@ __device__ __forceinline__ bool find_row_tile(const AttendPaged& a, uint32_t til
     for (uint32_t i = 0; i < a.p.sequences; i += 64u) {
         Sequence sq{};
         uint32_t tiles = 0;
-        if (i + lane < a.p.sequences && read_sequence(a.p, i + lane, sq) && sq.count * a.group.d > FEW_ROWS)
-            tiles = (sq.count * a.group.d + ROW_TILE - 1u) / ROW_TILE;
+        if (i + lane < a.p.sequences && read_sequence(a.p, i + lane, sq) && (a.alone || sq.count * a.group.d > FEW_ROWS))
+            tiles = (sq.count * a.group.d + a.row_tile - 1u) / a.row_tile;
         uint32_t through = tiles;
 #pragma unroll
         for (uint32_t d = 1; d < 64u; d <<= 1) {
@@ -804,35 +806,39 @@ __device__ __forceinline__ bool find_row_tile(const AttendPaged& a, uint32_t til
             w.sq.first = __builtin_amdgcn_readlane(sq.first, at);
             w.sq.count = __builtin_amdgcn_readlane(sq.count, at);
             w.sq.length = __builtin_amdgcn_readlane(sq.length, at);
-            return w.set(a, (__builtin_amdgcn_readlane(through, at) - 1u - tile) * ROW_TILE, ROW_TILE, part);
+            return w.set(a, (__builtin_amdgcn_readlane(through, at) - 1u - tile) * a.row_tile, a.row_tile, part);
         }
         tile -= __builtin_amdgcn_readlane(through, 63);
     }
     return false;
 }
 
-template <uint32_t KIND, uint32_t W>
+template <uint32_t KIND, uint32_t W, uint32_t KS>
 __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
-    typedef Tile<KIND, W> T;
+    typedef Tile<KIND, W, KS> T;
     constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ uint32_t redo[ROW_TILE / 32u];
+    __shared__ uint32_t redo[T::ROWS / 32u], cache_rows[2][KT];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
+    const uint32_t rows_of = wave % (4u / KS), keys_of = wave / (4u / KS);  // the wave's 32 rows, its share of the keys
     Rows w;
     uint32_t b = blockIdx.x;
     w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
     const uint32_t part = b % a.splits;
-    if (!find_row_tile(a, b / a.splits, part, w)) return;
+    if (!find_row_tile(a, b / a.splits, part, w)) {
+        if (a.alone && blockIdx.x == 0 && threadIdx.x == 0 && !read_sequence(a.p, 0, w.sq)) report(a.p.errors, 0, 1);
+        return;
+    }
     const uint32_t width = a.p.width;
     const size_t row_bytes = (size_t)width * Split<KIND>::BYTES;
 
     // this lane's query (rows past the tile's repeat its last), and the
     // positions of the wave's
-    const uint32_t r = w.first + min(wave * 32u + col, w.count - 1u);
+    const uint32_t r = w.first + min(rows_of * 32u + col, w.count - 1u);
     const uint32_t pos = w.position(a, r);
-    const bool idle = wave * 32u >= w.count;
-    const uint32_t lo = w.position(a, w.first + min(wave * 32u, w.count - 1u));
-    const uint32_t hi = w.position(a, w.first + min(wave * 32u + 31u, w.count - 1u));
+    const bool idle = rows_of * 32u >= w.count;
+    const uint32_t lo = w.position(a, w.first + min(rows_of * 32u, w.count - 1u));
+    const uint32_t hi = w.position(a, w.first + min(rows_of * 32u + 31u, w.count - 1u));
     Operand<NP> query[W / 16u];
     float power = 1.0f, undo = 1.0f;
     {
@@ -863,18 +869,19 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
 
     // step i: KT positions. A thread brings chunk at % CHUNKS of rows at /
     // CHUNKS for at = threadIdx.x + 256 l (where a row is narrower than W its
-    // first columns stand in); the pages of the rows are looked up a step ahead.
+    // first columns stand in). One wave in turn looks up the pages of a step's
+    // rows, two steps ahead.
     constexpr uint32_t PER = KEYS / KT;
     const uint32_t steps = PER * (w.end - w.begin);
     const auto first_key = [&](uint32_t i) { return w.span.key(w.begin + i / PER) + i % PER * KT; };
-    uint32_t rows[T::LOADS];
-    const auto look_up = [&](uint32_t i) {
+    const auto get_rows = [&](uint32_t i, uint32_t (&rows)[T::LOADS]) {
 #pragma unroll
-        for (uint32_t l = 0; l < T::LOADS; ++l)
-            rows[l] = w.cache_row_for(a, first_key(i) + (threadIdx.x + l * 256u) / T::CHUNKS);
+        for (uint32_t l = 0; l < T::LOADS; ++l) rows[l] = cache_rows[i & 1u][(threadIdx.x + l * 256u) / T::CHUNKS];
     };
-    const auto load_direct = [&](uint32_t buffer) {
-        const uint32_t to = lds_address(lds + buffer * T::STAGE + wave * 1024u);
+    const auto load_direct = [&](uint32_t i) {
+        uint32_t rows[T::LOADS];
+        get_rows(i, rows);
+        const uint32_t to = lds_address(lds + (i & 1u) * T::STAGE + wave * 1024u);
 #pragma unroll
         for (uint32_t l = 0; l < T::LOADS; ++l) {
             const uint32_t at = threadIdx.x + l * 256u;
@@ -885,7 +892,9 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         }
     };
     f32x4 held[T::F32 ? T::LOADS : 1][2][2];
-    const auto load_held = [&]() {
+    const auto load_held = [&](uint32_t i) {
+        uint32_t rows[T::LOADS];
+        get_rows(i, rows);
 #pragma unroll
         for (uint32_t l = 0; l < T::LOADS; ++l) {
             const uint32_t c = (threadIdx.x + l * 256u) % T::CHUNKS * 32u;
@@ -916,35 +925,39 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
     // In units of the scores times power: zero is what weights count from (the
     // reference less HEADROOM), limit the score that sets the reference anew.
     float zero = 0.0f, limit = -INFINITY, total = 0.0f;
+    const bool scaled = __any(undo != 1.0f);
     f32x16 out[W / 32u];
 #pragma unroll
     for (uint32_t d = 0; d < W / 32u; ++d) out[d] = f32x16{} * 0.0f;
-    if (threadIdx.x < ROW_TILE / 32u) redo[threadIdx.x] = 0;
-    look_up(0);
+    if (threadIdx.x < T::ROWS / 32u) redo[threadIdx.x] = 0;
+    if (threadIdx.x < 2u * KT && threadIdx.x / KT < steps)
+        cache_rows[threadIdx.x / KT][threadIdx.x % KT] = w.cache_row_for(a, first_key(threadIdx.x / KT) + threadIdx.x % KT);
+    lds_sync();
     if constexpr (T::F32)
-        load_held();
+        load_held(0);
     else
         load_direct(0);
-    if (steps > 1u) look_up(1);
     for (uint32_t i = 0; i < steps; ++i) {
         const uint8_t* stage = lds;
         if constexpr (T::F32) {
             lds_sync();  // the last step's tile has been read
             store_held();
             lds_sync();
-            if (i + 1u < steps) load_held();
+            if (i + 1u < steps) load_held(i + 1u);
         } else {
             // this step's tile has landed, and every wave is past the last's
             wait_vm_lds<0>();
             lds_sync();
-            if (i + 1u < steps) load_direct((i + 1u) & 1u);
+            if (i + 1u < steps) load_direct(i + 1u);
             stage = lds + (i & 1u) * T::STAGE;
         }
-        if (i + 2u < steps) look_up(i + 2u);
+        const bool looks = i + 2u < steps && wave == (i & 3u);
+        uint32_t ahead = 0;
+        if (looks) ahead = w.cache_row_for(a, first_key(i + 2u) + lane % KT);
         const uint32_t k0 = first_key(i);
 #pragma unroll
-        for (uint32_t g0 = 0; g0 < KT / 32u; g0 += T::AT_ONCE) {
-            const uint32_t kg0 = k0 + g0 * 32u;
+        for (uint32_t g1 = 0; g1 < KT / 32u; g1 += T::AT_ONCE * KS) {
+            const uint32_t g0 = g1 + keys_of, kg0 = k0 + g0 * 32u;
             // keys that none of the wave's rows sees
             if (idle || kg0 > hi || (kg0 >= a.sinks && kg0 + T::AT_ONCE * 32u <= window_start(a, lo))) continue;
             f32x16 scores[T::AT_ONCE];
@@ -985,13 +998,16 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
                         for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
                     }
                 }
+                score -= zero;
+                if (KIND == TMH_CACHE_F16 && scaled) {
+                    asm volatile("");  // a branch: most rows have no power
+                    score *= undo;
+                }
                 Operand<NP> weight[2];
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
-                    float e0 = score[j] - zero, e1 = score[j + 1] - zero;
-                    if (KIND == TMH_CACHE_F16) e0 *= undo, e1 *= undo;
-                    e0 = __builtin_amdgcn_exp2f(e0), e1 = __builtin_amdgcn_exp2f(e1);
+                    const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
                     sum += e0;
                     sum += e1;
                     split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
@@ -1016,16 +1032,48 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
                     }
             }
         }
+        if (looks && lane < KT) cache_rows[i & 1u][lane] = ahead;
     }
 
     total += __shfl_xor(total, 32, 64);
-    const uint32_t mine = wave * 32u + col;
-    if (mine < w.count) {
+    float top = limit == -INFINITY ? -INFINITY : zero * undo;
+    if constexpr (KS == 2u) {
+        // the rows' other half of the keys
+        float* other = (float*)lds + (rows_of * 64u + lane) * (W / 2u + 4u);
+        lds_sync();
+        if (keys_of == 1u) {
+#pragma unroll
+            for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e)
+                    *(f32x4*)(other + d * 16u + e * 4u) =
+                        f32x4{out[d][e * 4u], out[d][e * 4u + 1u], out[d][e * 4u + 2u], out[d][e * 4u + 3u]};
+            *(f32x4*)(other + W / 2u) = f32x4{top, total, 0.0f, 0.0f};
+        }
+        lds_sync();
+        if (keys_of == 0u) {
+            const f32x4 sums = *(const f32x4*)(other + W / 2u);
+            const float best = fmaxf(top, sums[0]), ref = best == -INFINITY ? 0.0f : best;
+            const float mine = __builtin_amdgcn_exp2f(top - ref), theirs = __builtin_amdgcn_exp2f(sums[0] - ref);
+            top = best;
+            total = total * mine + sums[1] * theirs;
+#pragma unroll
+            for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    const f32x4 o = *(const f32x4*)(other + d * 16u + e * 4u);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; ++j) out[d][e * 4u + j] = out[d][e * 4u + j] * mine + o[j] * theirs;
+                }
+        }
+    }
+    const uint32_t mine = rows_of * 32u + col;
+    if (keys_of == 0u && mine < w.count) {
         bool finite = total < INFINITY && (total > 0.0f || !w.sees_any(a, pos));
         const float by = w.parts == 1u ? 1.0f / total : 1.0f;
         const size_t at = w.place(a, r) + part;
         float* to = w.parts == 1u ? a.dst + (size_t)w.token(a, r) * a.ld_dst + w.head(a, r) * width : a.part + at * width;
-        if (w.parts > 1u && half == 0) a.part_sums[at] = make_float2(limit == -INFINITY ? -INFINITY : zero * undo, total);
+        if (w.parts > 1u && half == 0) a.part_sums[at] = make_float2(top, total);
 #pragma unroll
         for (uint32_t d = 0; d < W / 32u; ++d)
 #pragma unroll
@@ -1043,7 +1091,10 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         if (!finite) atomicOr(&redo[mine / 32u], 1u << mine % 32u);
     }
     __syncthreads();
-    if (redo[0] | redo[1] | redo[2] | redo[3]) plain_rows<KIND>(a, w, part, redo);
+    uint32_t any = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < T::ROWS / 32u; ++i) any |= redo[i];
+    if (any) plain_rows<KIND>(a, w, part, redo);
 }
 
 // Joins the parts of row r, by a wave: each part brought to the highest reference
@@ -1120,14 +1171,14 @@ __global__ __launch_bounds__(256) void k_attend_join_few(AttendPaged a, uint32_t
     join_row(a, w, r, lanes[threadIdx.x >> 6]);
 }
 
-// Joins a quarter of a row tile, eight rows a wave.
+// Joins a quarter of a row tile, a quarter of that a wave.
 __global__ __launch_bounds__(256) void k_attend_join_tile(AttendPaged a) {
     __shared__ f32x4 lanes[4][64];
     Rows w;
     w.kh = blockIdx.x % a.p.kv_heads;
     if (!find_row_tile(a, blockIdx.x / a.p.kv_heads, 0, w) || w.parts == 1u) return;
-    const uint32_t from = blockIdx.y * (ROW_TILE / 4u) + (threadIdx.x >> 6) * (ROW_TILE / 16u);
-    for (uint32_t i = from; i < min(from + ROW_TILE / 16u, w.count); ++i)
+    const uint32_t from = blockIdx.y * (a.row_tile / 4u) + (threadIdx.x >> 6) * (a.row_tile / 16u);
+    for (uint32_t i = from; i < min(from + a.row_tile / 16u, w.count); ++i)
         join_row(a, w, w.first + i, lanes[threadIdx.x >> 6]);
 }
 
@@ -1149,22 +1200,22 @@ void launch_few_of(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipS
         launch_few<KIND, 256>(a, row_tiles, grid, stream);
 }
 
-template <uint32_t KIND, uint32_t W>
+template <uint32_t KIND, uint32_t W, uint32_t KS>
 void launch_tile(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
-    constexpr uint32_t lds = Tile<KIND, W>::LDS;
-    TMH_LAUNCH((k_attend_tile<KIND, W>), dim3(grid), dim3(256), lds, stream, a);
+    constexpr uint32_t lds = Tile<KIND, W, KS>::LDS;
+    TMH_LAUNCH((k_attend_tile<KIND, W, KS>), dim3(grid), dim3(256), lds, stream, a);
 }
 
 template <uint32_t KIND>
 void launch_tile_of(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
     if (a.p.width <= 32u)
-        launch_tile<KIND, 32>(a, grid, stream);
+        a.row_tile == 128u ? launch_tile<KIND, 32, 1>(a, grid, stream) : launch_tile<KIND, 32, 2>(a, grid, stream);
     else if (a.p.width <= 64u)
-        launch_tile<KIND, 64>(a, grid, stream);
+        a.row_tile == 128u ? launch_tile<KIND, 64, 1>(a, grid, stream) : launch_tile<KIND, 64, 2>(a, grid, stream);
     else if (a.p.width <= 128u)
-        launch_tile<KIND, 128>(a, grid, stream);
+        launch_tile<KIND, 128, 1>(a, grid, stream);
     else
-        launch_tile<KIND, 256>(a, grid, stream);
+        launch_tile<KIND, 256, 1>(a, grid, stream);
 }
 
 // Tiles of keys that a row tile of `tokens` new tokens sees, at most.
@@ -1193,7 +1244,7 @@ hipError_t launch_attention_paged(const AttendPaged& few, uint32_t few_groups, u
             e = hipGetLastError();
         }
     }
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || more.alone) return e;
     launch_few_of<KIND>(few, row_tiles, few_groups * few.splits, stream);
     e = hipGetLastError();
     if (e == hipSuccess && few.splits > 1u) {
@@ -1276,22 +1327,27 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
     AttendPaged a{{(const int32_t*)page_table, (const int32_t*)starts, (const int32_t*)lengths, table_width, sequences,
                    tokens, max_new, max_length, pages, kv_heads, width, Divider(page_size), ctx.errors},
                   (const float*)q, ldq, heads, Divider(group), (const void*)keys, (const void*)values, window, sinks,
-                  (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst, 0, 1, 0, nullptr, nullptr};
+                  (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst, 0, 1, 0, 128, 0, nullptr, nullptr};
     // Few rows: shares of the keys such that four workgroups a compute unit
-    // have one each, of at least a step for each of their waves. More rows:
-    // two a compute unit, of at least eight tiles of keys.
+    // have one each, of at least eight tiles of keys (two steps a wave; a join
+    // costs more than that: 512 positions 9.0 us in two launches, 7.5 in one),
+    // or sixteen where there is a workgroup for each compute unit without (48
+    // windows of 1024: 114 -> 101 us). More rows: two a compute unit, of at least
+    // eight.
     AttendPaged few = a, more = a;
     const uint64_t rows = std::max<uint64_t>(1u, (uint64_t)max_new * group);
     few.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, rows);
     const uint32_t row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
     const uint64_t few_groups = (uint64_t)sequences * kv_heads * row_tiles;
     const uint64_t few_tiles = most_tiles(a, FEW_ROWS);
-    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, 2u);
+    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, few_groups > (uint32_t)ctx.compute_units ? 16u : 8u);
     const bool has_more = rows > FEW_ROWS;
+    more.row_tile = width <= 64u ? 64 : 128;
+    more.alone = has_more && sequences == 1u;  // one launch for the usual prompt
     // row tiles of all sequences, at most
     const uint64_t more_groups =
-        ((uint64_t)tokens * group / ROW_TILE + std::min<uint64_t>(sequences, (uint64_t)tokens * group / (FEW_ROWS + 1u))) * kv_heads;
-    if (has_more) set_shares(more, more_groups, most_tiles(a, ROW_TILE), 2u * ctx.compute_units, 8u);
+        ((uint64_t)tokens * group / more.row_tile + std::min<uint64_t>(sequences, more.alone ? 1u : (uint64_t)tokens * group / (FEW_ROWS + 1u))) * kv_heads;
+    if (has_more) set_shares(more, more_groups, most_tiles(a, more.row_tile), 2u * ctx.compute_units, 8u);
     if (few_groups * few.splits > 0x7fffffffull || more_groups * more.splits > 0x7fffffffull) return TMH_ERROR_SHAPE;
     const size_t few_parts = few.splits > 1u ? (size_t)sequences * kv_heads * few.room * few.splits : 0;
     const size_t more_parts = more.splits > 1u ? (size_t)tokens * heads * more.splits : 0;

@@ -10,10 +10,12 @@
 // looked up in it, and only few candidates are taken further: those through the
 // cut's bin where they fit the LDS, else those of that one bin.
 //
-// Weights are exp2 in f64, summed as integers of 2^-shift (shift = 62 less the
-// bits of n, at most 50: 45 at a vocabulary of 131071), so a sum is the same in
-// any order and the ids do not depend on how the work falls; a weight below
-// half that step counts as none.
+// Weights are exp2 in f64, to 2^-48 of each, and summed as integers, so a sum is
+// the same in any order and the ids do not depend on how the work falls. A bin
+// counts in units of its own, 2^-shift of the power of two above its weights
+// (shift = 62 less the bits of n, at most 50: 45 at a vocabulary of 131071);
+// sums over bins are in units of 2^-60 of the whole sum or less. Weights below
+// 2^-80 count as none.
 //
 // Three launches: chunks' highest and lowest values, chunks' histograms added
 // to their row's, then a workgroup a row. A row of 131072 takes about 30 vector
@@ -62,8 +64,9 @@ struct Extent {
 
 // A row's histogram.
 struct Histogram {
-    u64 sums[BINS];
-    u64 least;  // the sum of the weights that min_p leaves
+    u64 sums[BINS];  // each in its bin's units
+    u64 rough;       // their sum in the highest's units, each cut to whole ones
+    u64 least;       // of the weights that min_p leaves in the bin of its border
     uint32_t counts[BINS];
 };
 
@@ -91,6 +94,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key : key ^ 0x7fffffffu);
 }
 
+constexpr uint32_t MINUS_INFINITY = 0xff800000u;  // its key
+
+// v · 2^-by, by of either sign: shifted, and cut where bits fall out.
+__device__ __forceinline__ u64 scale_down(u64 v, int by) {
+    return by >= 64 ? 0 : by >= 0 ? v >> by : v << -by;
+}
+
 // 2^-y for y from 0 to 64: the exponent, and 2^f by its Taylor polynomial to
 // f^11 for f within half of 0 (off by less than 2^-46 of it).
 __device__ __forceinline__ double exp2_minus(double y) {
@@ -115,31 +125,35 @@ __device__ __forceinline__ double exp2_minus(double y) {
 // A row's measure: its highest value, and y's scale, end and bins.
 struct Measure {
     float highest, scale, cut, per_y;
-    double exact, bin_y, one;  // the scale in f64; a bin's y; 2^shift
+    double exact, bin_y;  // the scale in f64; a bin's y
+    uint32_t shift;
 
-    __device__ __forceinline__ Measure(const Extent& e, float temperature, uint32_t shift) {
+    __device__ __forceinline__ Measure(const Extent& e, float temperature, uint32_t bits) {
         highest = e.high;
         exact = 1.4426950408889634 / (double)temperature;
         scale = (float)exact;
-        cut = (float)(shift + 2u);
-        one = (double)((u64)1 << shift);
-        const float range = fminf((e.high - e.low) * scale, cut);
-        per_y = range > 0.0f ? fminf((float)BINS / range, 1e30f) : 0.0f;
-        bin_y = range > 0.0f ? 1.0 / (double)per_y : 0.0;
+        cut = fminf((e.high - e.low) * scale, 80.0f);  // the lowest's
+        shift = bits;
+        per_y = cut > 0.0f ? fminf((float)BINS / cut, 1e30f) : 0.0f;
+        bin_y = cut > 0.0f ? 1.0 / (double)per_y : 0.0;
     }
-    // y in f32 falls as x rises, so bins stand in the candidates' order, and
-    // y above cut is a weight of none. NaN and -inf are not within it.
+    // y in f32 falls as x rises, so bins stand in the candidates' order; y above
+    // cut is a weight of none, or no candidate's. NaN and -inf are not within it.
     __device__ __forceinline__ float y(float x) const { return x == highest ? 0.0f : (highest - x) * scale; }
     __device__ __forceinline__ bool within(float y) const { return y <= cut; }
     __device__ __forceinline__ uint32_t bin(float y) const { return min((uint32_t)(y * per_y), BINS - 1u); }
-    // A weight of 2^shift for the highest is that at the bin's beginning times
-    // 2^-rest, the rest of y (at most 52 / BINS) by its Taylor polynomial to
-    // the fifth power, off by less than 2^-44 of it.
-    __device__ __forceinline__ double begin(uint32_t bin) const { return exp2_minus((double)bin * bin_y) * one; }
+    // A bin's unit is 2^-(shift + power). A weight is that at the bin's beginning
+    // times 2^-rest, the rest of y (at most 80 / BINS) by its Taylor polynomial
+    // to the sixth power, off by less than 2^-48 of it.
+    __device__ __forceinline__ uint32_t power(uint32_t bin) const { return (uint32_t)((double)bin * bin_y); }
+    __device__ __forceinline__ double begin(uint32_t bin) const {
+        return exp2_minus((double)bin * bin_y - (double)power(bin)) * (double)((u64)1 << shift);
+    }
     __device__ __forceinline__ double scaled(float x, uint32_t bin, double begin) const {
         const double y = x == highest ? 0.0 : ((double)highest - (double)x) * exact;
         const double rest = __builtin_fma((double)bin, -bin_y, y);
-        double p = -0.0013333558146428443;  // (-ln 2)^k / k!
+        double p = 0.00015403530393381608;  // (-ln 2)^k / k!
+        p = __builtin_fma(p, rest, -0.0013333558146428443);
         p = __builtin_fma(p, rest, 0.009618129107628477);
         p = __builtin_fma(p, rest, -0.05550410866482158);
         p = __builtin_fma(p, rest, 0.2402265069591007);
@@ -151,27 +165,24 @@ struct Measure {
     static __device__ __forceinline__ u64 whole(double scaled) {
         return (u64)__builtin_bit_cast(long long, scaled + 4503599627370496.0) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ u64 weight(float x) const {
-        const uint32_t b = bin(y(x));
-        return whole(scaled(x, b, begin(b)));
+    __device__ __forceinline__ u64 weight(float x, uint32_t bin) const { return whole(scaled(x, bin, begin(bin))); }
+    __device__ __forceinline__ u64 weight(float x) const { return weight(x, bin(y(x))); }
+    // Whether the weight of x is at least `least` of the highest's.
+    __device__ __forceinline__ bool reaches(float x, float least) const {
+        const float v = y(x);
+        if (!within(v)) return false;
+        const uint32_t b = bin(v);
+        return scaled(x, b, begin(b)) >= __builtin_ldexp((double)least, (int)(shift + power(b)));
     }
-    // The first key whose bin is `from` or after it (keys not within cut are
-    // after all bins), by 64 keys a round: near where the bin should begin,
-    // else among all.
-    __device__ __forceinline__ bool past(uint32_t key, uint32_t from) const {
-        const float v = y(value_of(key));
-        return !within(v) || bin(v) >= from;
-    }
-    __device__ __forceinline__ uint32_t first_key(uint32_t from) const {
-        const uint32_t lane = threadIdx.x & 63u, first = key_of(highest), last = 0xff800000u;  // -inf's
-        const uint32_t guess = key_of(highest - (float)from / per_y / scale);
-        uint32_t low = max(first, guess - min(guess, 2048u)), high = min(last, guess + 2047u);
-        const bool near = low < high && (low == first || !past(low, from)) && (high == last || past(high, from));
-        if (!__all(near)) low = first, high = last;
+    // The first key (of a value not above the highest) for which `past` is true,
+    // by 64 keys a round; past is false, then true, and -inf's key is past.
+    template <class PAST>
+    __device__ __forceinline__ uint32_t search(uint32_t low, uint32_t high, PAST past) const {
+        const uint32_t lane = threadIdx.x & 63u;
         while (low < high) {
             const uint32_t step = (high - low - 1u) / 64u + 1u;
             const u64 at = (u64)low + (u64)step * lane;
-            const uint64_t ones = __ballot(at >= high || past((uint32_t)at, from));
+            const uint64_t ones = __ballot(at >= high || past((uint32_t)at));
             const uint32_t n = ones ? (uint32_t)__ffsll((unsigned long long)ones) - 1u : 64u;
             if (n == 0) return low;
             high = (uint32_t)min((u64)high, (u64)low + (u64)step * n);
@@ -179,13 +190,35 @@ struct Measure {
         }
         return low;
     }
+    // The first key whose bin is `from` or after it (keys not within cut are
+    // after all bins): near where the bin should begin, else among all.
+    __device__ __forceinline__ uint32_t first_key(uint32_t from) const {
+        const auto past = [&](uint32_t key) {
+            const float v = y(value_of(key));
+            return !within(v) || bin(v) >= from;
+        };
+        const uint32_t first = key_of(highest), guess = key_of(highest - (float)from / per_y / scale);
+        uint32_t low = max(first, guess - min(guess, 2048u)), high = min(MINUS_INFINITY, guess + 2047u);
+        const bool near = low < high && (low == first || !past(low)) && (high == MINUS_INFINITY || past(high));
+        if (!__all(near)) low = first, high = MINUS_INFINITY;
+        return search(low, high, past);
+    }
+    // The first key whose weight is below `least` of the highest's.
+    __device__ __forceinline__ uint32_t first_below(float least) const {
+        return search(key_of(highest), MINUS_INFINITY, [&](uint32_t key) { return !reaches(value_of(key), least); });
+    }
+    // The bin of a key, BINS where it is not within cut.
+    __device__ __forceinline__ uint32_t bin_of_key(uint32_t key) const {
+        const float v = y(value_of(key));
+        return key < MINUS_INFINITY && within(v) ? bin(v) : BINS;
+    }
 };
 
-// Where a count or a sum is reached: the bin, what stands before it, how many
-// it holds; then the candidate, and the sum through it.
+// Where a count or a sum is reached: the bin, what stands before it and what it
+// holds; then the candidate, and the sum through it.
 struct Found {
     uint32_t bin, count_before, count, index;
-    u64 sum_before, sum;
+    u64 sum_before, sum_of, sum;
 };
 
 struct Lds {
@@ -265,7 +298,8 @@ struct Bins {
         for (uint32_t i = 0; i < PER; ++i) {
             if (t.in(c, counts[i], s, sums[i])) {
                 l.found.bin = threadIdx.x * PER + i;
-                l.found.count_before = c, l.found.count = counts[i], l.found.sum_before = s;
+                l.found.count_before = c, l.found.count = counts[i];
+                l.found.sum_before = s, l.found.sum_of = sums[i];
             }
             c += counts[i], s += sums[i];
         }
@@ -327,15 +361,22 @@ __device__ __forceinline__ void list_values(Lds& l, const float* row, uint32_t n
 }
 
 // Candidates one a lane of a wave, with what stands before each in their order.
+// Their weights are in units of 2^-FINE, or where they are of one bin in its.
+constexpr int FINE = 56;
 struct Few {
     u64 mine, weight, sum;
     uint32_t n, count;
 
-    __device__ __forceinline__ Few(const u64* from, uint32_t size, const Measure& m, uint32_t before, u64 sum_before)
-        : sum(sum_before), n(size), count(before) {
+    __device__ __forceinline__ Few(const u64* from, uint32_t size, const Measure& m, bool one_bin, uint32_t before,
+                                   u64 sum_before)
+        : mine(~0ull), weight(0), sum(sum_before), n(size), count(before) {
         const uint32_t lane = threadIdx.x & 63u;
-        mine = lane < n ? from[lane] : ~0ull;
-        weight = lane < n ? m.weight(value_of((uint32_t)(mine >> 32))) : 0;
+        if (lane < n) {
+            mine = from[lane];
+            const float x = value_of((uint32_t)(mine >> 32));
+            const uint32_t bin = m.bin(m.y(x));
+            weight = scale_down(m.weight(x, bin), one_bin ? 0 : (int)(m.shift + m.power(bin)) - FINE);
+        }
         for (uint32_t j = 0; j < n; ++j) {
             const bool less = one(mine, j) < mine;
             count += less ? 1u : 0u;
@@ -390,7 +431,7 @@ __device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, 
     }
     __syncthreads();
     if (threadIdx.x < 64u) {
-        const Few few(l.few, n, m, count, sum);
+        const Few few(l.few, n, m, true, count, sum);
         u64 through;
         const uint32_t index = few.find(t, through);
         if (threadIdx.x == 0) l.found.index = index, l.found.sum = through;
@@ -398,10 +439,35 @@ __device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, 
     __syncthreads();
 }
 
+// The candidate that the target is in among those of the value of `key`, by index:
+// more of them than the list holds.
+__device__ __forceinline__ void find_equal(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, uint32_t key) {
+    const u64 sum = l.found.sum_before, weight = m.weight(value_of(key));
+    const u64 place = t.by_sum ? (t.target - sum) / weight : t.target - l.found.count_before;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < n; base += THREADS) {
+        const uint32_t j = base + threadIdx.x;
+        const bool is = j < n && key_of(row[j]) == key;
+        uint32_t c = is ? 1u : 0u, all;
+        u64 s = 0, total;
+        scan(l, c, s, all, total);
+        if (is && before + c == place) l.found.index = j, l.found.sum = sum + (place + 1u) * weight;
+        before += all;
+    }
+    __syncthreads();
+}
+
 // The candidate that the target is in, and the sum through it, into l.found;
-// the target's bin is there. `listed`: the bin's candidates are.
-__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, bool listed) {
+// the target's bin is there, and its sum in its own units in `held`, `finer` bits
+// below the common ones. `listed`: the bin's candidates are.
+__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, u64 held,
+                                            int finer, bool listed) {
     uint32_t low = m.first_key(l.found.bin), high = m.first_key(l.found.bin + 1u) - 1u;
+    const u64 common_before = l.found.sum_before, common = l.found.sum_of;
+    __syncthreads();
+    if (threadIdx.x == 0) l.found.sum_before = 0;
+    if (t.by_sum) t.target = min(scale_down(t.target - common_before, -finer), held - 1u);
+    __syncthreads();
     // more than the list holds: histograms of ever fewer keys
     while (l.found.count > LIST && low < high) {
         uint32_t shift = 0;
@@ -421,29 +487,15 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
         low += l.found.bin << shift;
         high = min(high, low + (1u << shift) - 1u);
     }
-    const uint32_t count = l.found.count_before;
-    const u64 sum = l.found.sum_before;
     if (l.found.count <= LIST) {
         if (!listed) list_values(l, row, n, value_of(high), value_of(low));
         find_listed(l, m, t, low, high);
-        return;
+    } else {
+        find_equal(l, m, row, n, t, low);
     }
-    // one value more often than the list holds: by index
-    const u64 weight = m.weight(value_of(low));
-    const u64 place = t.by_sum ? (t.target - sum) / weight : t.target - count;
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < n; base += THREADS) {
-        const uint32_t j = base + threadIdx.x;
-        const bool is = j < n && key_of(row[j]) == low;
-        uint32_t c = is ? 1u : 0u, all;
-        u64 s = 0, total;
-        scan(l, c, s, all, total);
-        if (is && before + c == place) l.found.index = j, l.found.sum = sum + (place + 1u) * weight;
-        before += all;
-    }
+    if (threadIdx.x == 0) l.found.sum = common_before + min(scale_down(l.found.sum, finer), common);
     __syncthreads();
 }
-
 // The highest and lowest values of chunk blockIdx.y of row blockIdx.x, whose
 // share of the row's histogram it clears. Rows stand first in the grid, up to
 // a multiple of eight: a row's chunks then meet on one XCD, whose L2 holds the
@@ -462,7 +514,7 @@ __global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
     });
     Histogram& h = a.rows[r];
     for (uint32_t b = chunk * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
-    if (chunk == 0 && threadIdx.x == 0) h.least = 0;
+    if (chunk == 0 && threadIdx.x == 0) h.least = 0, h.rough = 0;
     e.take_wave();
     if (lane == 0) waves[wave] = e;
     __syncthreads();
@@ -493,7 +545,8 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     Extent e;
     if (!row_extent(a, r, temperature, e)) return;
     const Measure m(e, temperature, a.shift);
-    const double least = a.min_p ? (double)a.min_p[r] * m.one : 0.0;
+    const float least = a.min_p ? a.min_p[r] : 0.0f;
+    const uint32_t below = least <= 0.0f ? MINUS_INFINITY : m.first_below(least), border = m.bin_of_key(below);
 #pragma unroll
     for (uint32_t i = 0; i < BINS / THREADS; ++i) {
         const uint32_t b = threadIdx.x + i * THREADS;
@@ -501,7 +554,6 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     }
     if (threadIdx.x == 0) least_sum = 0;
     __syncthreads();
-    const bool cut_least = !(least <= 0.0);
     u64 kept = 0;
     each_value<4>(row, blockIdx.y * a.chunk, min(blockIdx.y * a.chunk + a.chunk, a.n), [&](float x, uint32_t) {
         const float y = m.y(x);
@@ -511,10 +563,10 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
             const u64 weight = m.whole(scaled);
             atomicAdd(&counts[bin], 1u);
             atomicAdd(&sums[bin], weight);
-            if (cut_least && scaled >= least) kept += weight;
+            if (bin == border && key_of(x) < below) kept += weight;
         }
     });
-    if (cut_least) {
+    if (border < BINS) {
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) kept += __shfl_xor(kept, d, 64);
         if ((threadIdx.x & 63u) == 0) atomicAdd(&least_sum, kept);
@@ -522,9 +574,11 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     __syncthreads();
     Histogram& h = a.rows[r];
     if (threadIdx.x == 0 && least_sum) atomicAdd(&h.least, least_sum);
+    u64 rough = 0;
 #pragma unroll
     for (uint32_t i = 0; i < BINS / THREADS; ++i) {
         const uint32_t b = threadIdx.x + i * THREADS;
+        rough += scale_down(sums[b], (int)m.power(b));
         if (a.chunks == 1u) {
             h.counts[b] = counts[b], h.sums[b] = sums[b];
         } else if (counts[b]) {
@@ -532,6 +586,9 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
             if (sums[b]) atomicAdd(&h.sums[b], sums[b]);
         }
     }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) rough += __shfl_xor(rough, d, 64);
+    if ((threadIdx.x & 63u) == 0) atomicAdd(&h.rough, rough);
 }
 
 // One row by one workgroup: the cuts and the choice.
@@ -552,47 +609,69 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
     const Measure m(e, temperature, a.shift);
     constexpr uint32_t PER = BINS / THREADS;
     const Histogram& h = a.rows[r];
+    // Common units of 2^-common: the sum of all weights, less than twice what it
+    // roughly is, stays below 2^62 of them. A bin's own are finer by so many bits.
+    const int bits = 65 - __clzll((long long)h.rough), common = 62 + (int)m.shift - bits;
+    const auto finer = [&](uint32_t bin) { return (int)(m.shift + m.power(bin)) - common; };
     Bins<PER> bins;
     bins.count_before = 0, bins.sum_before = 0;
 #pragma unroll
     for (uint32_t i = 0; i < PER; ++i) {
-        bins.counts[i] = h.counts[threadIdx.x * PER + i], bins.sums[i] = h.sums[threadIdx.x * PER + i];
+        const uint32_t b = threadIdx.x * PER + i;
+        bins.counts[i] = h.counts[b], bins.sums[i] = scale_down(h.sums[b], finer(b));
         bins.count_before += bins.counts[i], bins.sum_before += bins.sums[i];
     }
     const float least = a.min_p ? a.min_p[r] : 0.0f, p = a.top_p ? a.top_p[r] : 1.0f, u = a.u[r];
     const int32_t k = a.top_k ? a.top_k[r] : 0;
-    const u64 least_sum = h.least;
     uint32_t all;
     u64 total;
     scan(l, bins.count_before, bins.sum_before, all, total);
     // the prefix that stays is the shortest of three: the sums through the
     // k-th, through the first to reach p, and of weights of at least min_p
-    const bool cut_k = k > 0 && (uint32_t)k < all, cut_p = !(p >= 1.0f), cut_least = !(least <= 0.0f);
+    const bool cut_k = k > 0 && (uint32_t)k < all, cut_p = !(p >= 1.0f);
+    u64 least_sum = ~0ull;
+    if (!(least <= 0.0f)) {
+        const uint32_t border = m.bin_of_key(m.first_below(least));
+        if (border < BINS) {
+            __syncthreads();
+            if (threadIdx.x == border / PER) {
+                u64 before = bins.sum_before;
+#pragma unroll
+                for (uint32_t i = 0; i < PER; ++i) before += threadIdx.x * PER + i < border ? bins.sums[i] : 0;
+                l.found.sum = before + scale_down(h.least, finer(border));
+            }
+            __syncthreads();
+            least_sum = l.found.sum;
+        }
+    }
     const Target kth{false, (u64)k - 1u};
-    const auto reach = [&](u64 of) {
-        const double sum = (double)p * (double)of;
+    // the first to reach p of a sum, the first to pass u of it
+    const auto reach = [&](double of) {
+        const double sum = (double)p * of;
         return Target{true, sum > 0.0 ? (u64)__builtin_ceil(sum) - 1u : 0};
     };
     const auto choice = [&](u64 of) {
         const double sum = (double)u * (double)of;
         return Target{true, sum > 0.0 ? min((u64)sum, of - 1u) : sum == sum ? 0 : of - 1u};
     };
-    const u64 first = (u64)1 << a.shift;  // the highest's weight: it always stays
     bool listed = false;
     if (cut_k || cut_p) {
-        bins.find(l, cut_k ? kth : reach(total));
+        bins.find(l, cut_k ? kth : reach((double)total));
         if (l.found.count_before + l.found.count <= LIST) {
             // the candidates through the cut's bin: of them from here on
             listed = true;
             list_values(l, row, n, value_of(m.first_key(l.found.bin + 1u) - 1u), m.highest);
             if (l.listed <= FEW) {
                 if (threadIdx.x < 64u) {
-                    const Few few(l.list, l.listed, m, 0, 0);
-                    u64 through;
-                    if (cut_k) few.find(kth, total);
-                    if (cut_p) few.find(reach(total), through), total = min(total, through);
-                    if (cut_least) total = min(total, least_sum);
-                    const uint32_t index = few.find(choice(max(total, first)), through);
+                    // in units of 2^-FINE
+                    const Few few(l.list, l.listed, m, false, 0, 0);
+                    u64 through, left = ~0ull;
+                    double of = __builtin_ldexp((double)total, FINE - common);
+                    if (cut_k) few.find(kth, left), of = (double)left;
+                    if (cut_p) few.find(reach(of), through), left = min(left, through);
+                    if (least_sum != ~0ull)
+                        left = min(left, (u64)fmin(__builtin_ldexp((double)least_sum, FINE - common), 9.0e18));
+                    const uint32_t index = few.find(choice(max(left, (u64)1 << FINE)), through);
                     if (threadIdx.x == 0) a.ids[r] = (int32_t)index;
                 }
                 return;
@@ -601,12 +680,14 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
     }
     const auto find = [&](Target t) {
         bins.find(l, t);
-        find_in_bin(l, m, row, n, t, listed);
+        const uint32_t bin = l.found.bin;
+        find_in_bin(l, m, row, n, t, h.sums[bin], finer(bin), listed);
     };
     if (cut_k) find(kth), total = l.found.sum;
-    if (cut_p) find(reach(total)), total = min(total, l.found.sum);
-    if (cut_least) total = min(total, least_sum);
-    find(choice(max(total, first)));
+    if (cut_p) find(reach((double)total)), total = min(total, l.found.sum);
+    total = min(total, least_sum);
+    // the highest always stays
+    find(choice(max(total, scale_down((u64)1 << m.shift, (int)m.shift - common))));
     if (threadIdx.x == 0) a.ids[r] = (int32_t)l.found.index;
 }
 

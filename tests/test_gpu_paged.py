@@ -359,3 +359,190 @@ def test_a_server_of_three_sequences(dev):
             assert chosen[s] == ref.sample(logits[s], u[s], t[s], top[s], p[s])
             ids[s].append(int(chosen[s]))
         new = [1, 1, 1]
+
+
+# ------------------------------------------------ what a caller may do besides
+
+@pytest.mark.parametrize("kind", ["F32", "F16", "BF16"])
+@pytest.mark.parametrize("count,length", [(1, 1), (40, 40), (3, 1000), (200, 1000), (64, 64), (65, 129)])
+@pytest.mark.parametrize("width", [64, 128])
+def test_one_sequence_of_any_count(dev, kind, count, length, width):
+    # one sequence alone, with max_new well above what it has
+    say("one sequence", kind, count, length, width)
+    batch = ref.Batch([(count, length)], 16, seed=30, lead=3, trail=5)
+    q, keys, values = inputs(31, batch, 4, 2, width)
+    cache, k, v = cache_of(dev, kind, batch, 2, keys, values)
+    b = batch.on(dev)
+    b.max_new, b.max_length = 300, 5000
+    dst = dev.from_array(np.full(q.shape, 7.25, np.float32))
+    dev.attention_paged(dev.from_array(q), batch.tokens, 4, cache, b, 0.125, dst=dst)
+    got = dev.to_array(dst, np.float32, q.size).reshape(q.shape)
+    dev.sync()
+    want, tol = ref.attention(q, k, v, batch, 0.125)
+    agree(got, want, tol, batch)
+
+
+@pytest.mark.parametrize("kind", ["F32", "F16", "BF16"])
+def test_many_heads_of_one_kv_head(dev, kind):
+    # a single token's query rows fill more than a tile of few rows
+    say("heads", kind)
+    batch = ref.Batch([(1, 70), (1, 300), (3, 65)], 32, seed=32)
+    for heads in (17, 33, 71):
+        q, keys, values = inputs(33, batch, heads, 1, 64)
+        agree(*attend(dev, kind, batch, q, keys, values), batch)
+
+
+def test_pages_of_hidden_positions_may_be_gone(dev):
+    # a server frees what has left the window: those entries are no pages, and are not looked at
+    window, sinks, ps = 40, 5, 16
+    for sequences in ([(1, 700), (1, 200), (20, 333), (90, 400)], [(100, 600)]):
+        say("gone", sequences)
+        batch = ref.Batch(sequences, ps, seed=34)
+        q, keys, values = inputs(35, batch, 4, 2, 64)
+        full = batch.table.copy()
+        for s, (c, n) in enumerate(sequences):
+            seen = np.zeros(n, bool)
+            for i in range(c):
+                seen |= ref.visible(n - c + i, np.arange(n), window, sinks)
+            for page in range(-(-n // ps)):
+                if not seen[page * ps:(page + 1) * ps].any():
+                    batch.table[s, page] = -1
+        assert (batch.table != full).any()
+        cache, k, v = cache_of(dev, "F16", batch, 2, keys, values)
+        dst = dev.from_array(np.full(q.shape, 7.25, np.float32))
+        dev.attention_paged(dev.from_array(q), batch.tokens, 4, cache, batch.on(dev), 0.125, window=window, sinks=sinks,
+                            dst=dst)
+        got = dev.to_array(dst, np.float32, q.size).reshape(q.shape)
+        dev.sync()  # no index error
+        batch.table = full
+        want, tol = ref.attention(q, k, v, batch, 0.125, window, sinks)
+        agree(got, want, tol, batch)
+
+
+def test_new_tokens_where_none_were_announced(dev):
+    batch = ref.Batch([(1, 20), (1, 30)], 16, seed=36)
+    q, keys, values = inputs(37, batch, 4, 2, 64)
+    cache, _, _ = cache_of(dev, "F16", batch, 2, keys, values)
+    for alone in (False, True):
+        say("unannounced", alone)
+        b = batch.on(dev)
+        b.max_new = 0
+        if alone:
+            b.sequences, b.max_new, b.max_length = 1, 40, 19
+        dst = dev.from_array(np.full(q.shape, 7.25, np.float32))
+        dev.attention_paged(dev.from_array(q), batch.tokens, 4, cache, b, 0.125, dst=dst)
+        got = dev.to_array(dst, np.float32, q.size)
+        with pytest.raises(th.ExecutionError):
+            dev.sync()
+        assert (got == 7.25).all()
+
+
+@pytest.mark.parametrize("kind,width", [("F32", 256), ("F16", 128)])
+def test_a_cache_past_four_gigabytes(dev, kind, width):
+    # pages at both ends of keys and values of more than 2^32 bytes each, and of more than 2^31 elements
+    ps, size = 64, 4 if kind == "F32" else 2
+    pages = (1 << 32) // (ps * width * size) + 400
+    say("past 4 GB", kind, width, pages)
+    batch = ref.Batch([(1, 150), (40, 200)], ps, seed=38, spare=0)
+    q, keys, values = inputs(39, batch, 2, 1, width)
+    small, k, v = cache_of(dev, kind, batch, 1, keys, values)
+    big = dev.paged_cache(kind, pages, ps, 1, width)
+    page = ps * width * size
+    where = np.array([0, pages - 1, pages - 2, 1, pages - 5, pages - 3, pages - 4], np.int32)[:batch.pages]
+    for i, at in enumerate(where):
+        for name in ("keys", "values"):
+            dev.copy(getattr(big, name), getattr(small, name), page, dst_offset=int(at) * page, src_offset=i * page)
+    want, tol = ref.attention(q, k, v, batch, 0.125)
+    held = batch.table.copy()
+    batch.table = np.where(held >= 0, where[np.maximum(held, 0)], held).astype(np.int32)
+    dst = dev.from_array(np.full(q.shape, 7.25, np.float32))
+    dev.attention_paged(dev.from_array(q), batch.tokens, 2, big, batch.on(dev), 0.125, dst=dst)
+    got = dev.to_array(dst, np.float32, q.size).reshape(q.shape)
+    agree(got, want, tol, batch)
+    # and a write there
+    x = np.random.default_rng(40).normal(0, 1, (batch.tokens, 4 * width)).astype(np.float32)
+    cos, sin = tables(200, width)
+    dev.rope_write_paged(dev.from_array(x), 4 * width, batch.tokens, 2, dev.from_array(cos), dev.from_array(sin), 200, big,
+                         batch.on(dev))
+    last, place = batch.slots(1)
+    out = dev.alloc(page)
+    dev.copy(out, big.values, page, src_offset=int(last[199]) * page)
+    row = ref.from_bits(dev.to_array(out, np.uint8, page), kind).reshape(ps, width)[place[199]]
+    dev.sync()
+    assert np.array_equal(row, ref.to_kind(x[-1, 3 * width:], kind)[1])
+    for b in (big.keys, big.values):
+        b.release()
+    dev.set_pool_limit(0)
+    dev.sync()  # gives the memory back
+    dev.set_pool_limit(1 << 30)
+
+
+def test_the_same_bits_on_every_call(dev):
+    batch = ref.Batch([(1, 3000), (1, 700), (200, 900)], 16, seed=41)
+    q, keys, values = inputs(42, batch, 8, 2, 64)
+    first = None
+    for _ in range(4):
+        say("again")
+        got, _, _ = attend(dev, "F16", batch, q, keys, values, window=500, sinks=4)
+        first = got if first is None else first
+        assert np.array_equal(got.view(np.uint32), first.view(np.uint32))
+
+
+def test_two_threads(dev):
+    # both need the library's scratch, of different sizes
+    import threading
+    jobs = []
+    for seed, sequences, heads in ((50, [(1, 5000), (1, 200)], 4), (51, [(120, 2000), (1, 900)], 8)):
+        batch = ref.Batch(sequences, 16, seed=seed)
+        q, keys, values = inputs(seed, batch, heads, 2, 64)
+        cache, k, v = cache_of(dev, "F16", batch, 2, keys, values)
+        jobs.append((batch, heads, cache, dev.from_array(q), q.shape, ref.attention(q, k, v, batch, 0.125)))
+    wrong = []
+
+    def work(job):
+        batch, heads, cache, q, shape, (want, tol) = job
+        dev.bind()
+        b = batch.on(dev)
+        for _ in range(10):
+            out = dev.attention_paged(q, batch.tokens, heads, cache, b, 0.125)
+            got = dev.to_array(out, np.float32, int(np.prod(shape))).reshape(shape)
+            if not (np.abs(got - want).max(-1) <= tol).all():
+                wrong.append(heads)
+
+    say("threads")
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=100)
+    assert not wrong and not any(t.is_alive() for t in threads)
+    dev.sync()
+
+
+def test_no_memory_and_no_kernels(dev):
+    # a growth of the scratch that fails is an error, and the next call has its scratch: this
+    # call's parts, 4096 x 8 rows of 256 in two, are more than any other test's here
+    tokens, heads, width, ps = 4096, 8, 256, 512
+    batch = ref.Batch([(tokens, tokens)], ps, seed=52)
+    zeros = dev.from_array(np.zeros((batch.pages, heads, ps, width), np.float16))
+    cache = dev.paged_cache("F16", batch.pages, ps, heads, width, keys=zeros, values=zeros)
+    q = np.random.default_rng(53).normal(0, 1, (tokens, heads, width)).astype(np.float32)
+    b, qb, dst = batch.on(dev), dev.from_array(q), dev.from_array(np.ones_like(q))
+    say("no memory")
+    dev.lib.tmh_debug_disable_kernels(1)
+    try:
+        with pytest.raises(th.NoKernels):
+            dev.attention_paged(qb, tokens, heads, cache, b, 0.125, dst=dst)
+    finally:
+        dev.lib.tmh_debug_disable_kernels(0)
+    dev.lib.tmh_debug_fail_allocations(1)
+    try:
+        with pytest.raises(th.DeviceError, match="OUT_OF_MEMORY"):
+            dev.attention_paged(qb, tokens, heads, cache, b, 0.125, dst=dst)
+    finally:
+        dev.lib.tmh_debug_fail_allocations(0)
+    assert (dev.to_array(dst, np.float32, q.size) == 1.0).all()
+    dev.attention_paged(qb, tokens, heads, cache, b, 0.125, dst=dst)
+    got = dev.to_array(dst, np.float32, q.size)
+    dev.sync()
+    assert (got == 0.0).all()

@@ -149,3 +149,55 @@ def test_frequencies(dev):
     u = ((np.arange(4096) + 0.5) / 4096).astype(np.float32)
     counts = np.bincount(run(dev, x, u), minlength=4)
     assert np.abs(counts - 4096 * np.array([0.5, 0.25, 0.15, 0.1])).max() <= 1.0
+
+
+def test_no_temperature_is_argmax(dev):
+    say("greedy")
+    rng = np.random.default_rng(12)
+    x = rng.integers(-4, 5, (40, 7001)).astype(np.float32)
+    x[3, 0] = np.nan
+    x[4] = np.nan
+    x[5, 1:] = np.nan
+    x[6] = -np.inf
+    x[7, 100] = np.inf
+    buf = dev.from_array(x)
+    want = dev.to_array(dev.argmax(buf, 40, 7001), np.int32, 40)
+    for t in (0.0, -1.0, np.nan):
+        got = run(dev, x, np.full(40, 0.7, np.float32), np.full(40, t, np.float32), k=np.full(40, 9, np.int32))
+        assert list(got) == list(want)
+
+
+def test_rows_past_four_gigabytes(dev):
+    rows, n, ldx = 3, 5000, 700000000
+    say("past 4 GB")
+    rng = np.random.default_rng(13)
+    x = rng.normal(0, 2, (rows, n)).astype(np.float32)
+    big, small = dev.alloc(4 * ((rows - 1) * ldx + n)), dev.from_array(x)
+    for r in range(rows):
+        dev.copy(big, small, 4 * n, dst_offset=4 * r * ldx, src_offset=4 * r * n)
+    u = np.array([0.2, 0.5, 0.9], np.float32)
+    got = dev.to_array(dev.sample(big, rows, n, dev.from_array(u), ldx=ldx), np.int32, rows)
+    dev.sync()
+    assert list(got) == [ref.sample(x[r], u[r]) for r in range(rows)]
+    big.release()
+    dev.set_pool_limit(0)
+    dev.sync()
+    dev.set_pool_limit(1 << 30)
+
+
+def test_lists_of_every_length(dev):
+    # top-k at the sizes where the candidates change hands: a wave's, the list's, the histogram's finer ones
+    say("lists")
+    rng = np.random.default_rng(14)
+    n = 60000
+    x = rng.normal(0, 3, n).astype(np.float32)
+    k = np.array([1, 2, 63, 64, 65, 66, 255, 1023, 1024, 1025, 4000, 4095, 4096, 4097, 8000, 59999], np.int32)
+    rows = k.size
+    x = np.stack([rng.permutation(x) for _ in range(rows)])
+    for u in (0.0, 0.37, 0.99, np.float32(1) - np.float32(2.0 ** -24)):
+        for p in (1.0, 0.97):
+            us, ps = np.full(rows, u, np.float32), np.full(rows, p, np.float32)
+            for t in (0.5, 5.0):
+                ts = np.full(rows, t, np.float32)
+                got = run(dev, x, us, ts, k, ps)
+                assert list(got) == [ref.sample(x[r], u, t, k[r], p) for r in range(rows)]

@@ -17,11 +17,11 @@
 // sums over bins are in units of 2^-60 of the whole sum or less. Weights below
 // 2^-80 count as none.
 //
-// Three launches: chunks' highest and lowest values, chunks' histograms added
-// to their row's, then a workgroup a row. A row of 131072 takes about 30 vector
-// operations a value for its weights and is read three times, from the caches
-// after the first; rows are cut in chunks until there is one for each compute
-// unit.
+// Few rows go in three launches: chunks' highest and lowest values, chunks'
+// histograms added to their row's, then a workgroup a row; rows are cut in chunks
+// until there is one for each compute unit. Many rows go a workgroup each, in one
+// launch. The weights' vector operations, about 40 a value, bound the histogram;
+// latencies, scans and the passes over the row the rest.
 #include "../../include/tensomite_hip.h"
 #include "tmh_device.h"
 #include "tmh_internal.h"
@@ -228,6 +228,7 @@ struct Lds {
     uint32_t zoom_counts[ZOOM];
     u64 wave_sum[WAVES];
     uint32_t wave_count[WAVES];
+    Extent waves[WAVES];
     Found found;
     uint32_t listed, picked;
 };
@@ -319,39 +320,45 @@ __device__ __forceinline__ void find_zoomed(Lds& l, Target t, uint32_t count, u6
     bins.find(l, t);
 }
 
-// Hands every value of row [from, to) with its index to `take`, over the
-// workgroup: four a load (of any alignment), AHEAD loads a thread in flight.
 struct alignas(4) Values {
     float v[4];
 };
 
-template <uint32_t AHEAD, class TAKE>
-__device__ __forceinline__ void each_value(const float* row, uint32_t from, uint32_t to, TAKE take) {
-    constexpr uint32_t STEP = 4u * THREADS;
-    uint32_t j = from + 4u * threadIdx.x;
-    for (; j + (AHEAD - 1u) * STEP + 4u <= to; j += AHEAD * STEP) {
-        Values x[AHEAD];
+// A row, or a chunk of it, in memory: each() hands every value with its index to
+// `take`, over the workgroup, four a load (of any alignment), AHEAD loads a
+// thread in flight.
+struct InMemory {
+    const float* row;
+    uint32_t from, to;
+
+    template <uint32_t AHEAD, class TAKE>
+    __device__ __forceinline__ void each(TAKE take) const {
+        constexpr uint32_t STEP = 4u * THREADS;
+        uint32_t j = from + 4u * threadIdx.x;
+        for (; j + (AHEAD - 1u) * STEP + 4u <= to; j += AHEAD * STEP) {
+            Values x[AHEAD];
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) x[i] = *reinterpret_cast<const Values*>(row + j + i * STEP);
+            for (uint32_t i = 0; i < AHEAD; ++i) x[i] = *reinterpret_cast<const Values*>(row + j + i * STEP);
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i)
+            for (uint32_t i = 0; i < AHEAD; ++i)
 #pragma unroll
-            for (uint32_t k = 0; k < 4u; ++k) take(x[i].v[k], j + i * STEP + k);
+                for (uint32_t k = 0; k < 4u; ++k) take(x[i].v[k], j + i * STEP + k);
+        }
+        for (; j + 4u <= to; j += STEP) {
+            const Values x = *reinterpret_cast<const Values*>(row + j);
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k) take(x.v[k], j + k);
+        }
+        for (; j < to; ++j) take(row[j], j);
     }
-    for (; j + 4u <= to; j += STEP) {
-        const Values x = *reinterpret_cast<const Values*>(row + j);
-#pragma unroll
-        for (uint32_t k = 0; k < 4u; ++k) take(x.v[k], j + k);
-    }
-    for (; j < to; ++j) take(row[j], j);
-}
+};
 
 // Lists the candidates with values from `low` to `high`: all of them counted in
 // l.listed, LIST at most in the list.
-__device__ __forceinline__ void list_values(Lds& l, const float* row, uint32_t n, float low, float high) {
+__device__ __forceinline__ void list_values(Lds& l, const InMemory& row, float low, float high) {
     if (threadIdx.x == 0) l.listed = 0;
     __syncthreads();
-    each_value<8>(row, 0, n, [&](float x, uint32_t j) {
+    row.each<8>([&](float x, uint32_t j) {
         if (x >= low && x <= high) {
             const uint32_t at = atomicAdd(&l.listed, 1u);
             if (at < LIST) l.list[at] = (u64)key_of(x) << 32 | j;
@@ -441,13 +448,13 @@ __device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, 
 
 // The candidate that the target is in among those of the value of `key`, by index:
 // more of them than the list holds.
-__device__ __forceinline__ void find_equal(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, uint32_t key) {
+__device__ __forceinline__ void find_equal(Lds& l, const Measure& m, const InMemory& row, Target t, uint32_t key) {
     const u64 sum = l.found.sum_before, weight = m.weight(value_of(key));
     const u64 place = t.by_sum ? (t.target - sum) / weight : t.target - l.found.count_before;
     uint32_t before = 0;
-    for (uint32_t base = 0; base < n; base += THREADS) {
+    for (uint32_t base = 0; base < row.to; base += THREADS) {
         const uint32_t j = base + threadIdx.x;
-        const bool is = j < n && key_of(row[j]) == key;
+        const bool is = j < row.to && key_of(row.row[j]) == key;
         uint32_t c = is ? 1u : 0u, all;
         u64 s = 0, total;
         scan(l, c, s, all, total);
@@ -460,8 +467,8 @@ __device__ __forceinline__ void find_equal(Lds& l, const Measure& m, const float
 // The candidate that the target is in, and the sum through it, into l.found;
 // the target's bin is there, and its sum in its own units in `held`, `finer` bits
 // below the common ones. `listed`: the bin's candidates are.
-__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const float* row, uint32_t n, Target t, u64 held,
-                                            int finer, bool listed) {
+__device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const InMemory& row, Target t, u64 held, int finer,
+                                            bool listed) {
     uint32_t low = m.first_key(l.found.bin), high = m.first_key(l.found.bin + 1u) - 1u;
     const u64 common_before = l.found.sum_before, common = l.found.sum_of;
     __syncthreads();
@@ -475,7 +482,7 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
         __syncthreads();
         l.zoom_counts[threadIdx.x] = 0, l.zoom_sums[threadIdx.x] = 0;
         __syncthreads();
-        each_value<4>(row, 0, n, [&](float x, uint32_t) {
+        row.each<4>([&](float x, uint32_t) {
             const uint32_t key = key_of(x);
             if (key >= low && key <= high) {
                 atomicAdd(&l.zoom_counts[(key - low) >> shift], 1u);
@@ -488,127 +495,89 @@ __device__ __forceinline__ void find_in_bin(Lds& l, const Measure& m, const floa
         high = min(high, low + (1u << shift) - 1u);
     }
     if (l.found.count <= LIST) {
-        if (!listed) list_values(l, row, n, value_of(high), value_of(low));
+        if (!listed) list_values(l, row, value_of(high), value_of(low));
         find_listed(l, m, t, low, high);
     } else {
-        find_equal(l, m, row, n, t, low);
+        find_equal(l, m, row, t, low);
     }
     if (threadIdx.x == 0) l.found.sum = common_before + min(scale_down(l.found.sum, finer), common);
     __syncthreads();
 }
-// The highest and lowest values of chunk blockIdx.y of row blockIdx.x, whose
-// share of the row's histogram it clears. Rows stand first in the grid, up to
-// a multiple of eight: a row's chunks then meet on one XCD, whose L2 holds the
-// row for the later launches.
-__global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
-    __shared__ Extent waves[WAVES];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t r = blockIdx.x, chunk = blockIdx.y;
-    if (r >= a.count) return;
-    const float* row = a.x + (size_t)r * a.ldx;
-    const uint32_t from = chunk * a.chunk, to = min(from + a.chunk, a.n);
+// The highest and lowest values of a row or chunk, into `waves`: every wave's.
+__device__ __forceinline__ void find_extent(Extent* waves, const InMemory& row) {
     Extent e{-INFINITY, INFINITY, ~0u};
-    each_value<4>(row, from, to, [&](float x, uint32_t j) {
+    row.each<4>([&](float x, uint32_t j) {
         if (x == x && (e.index == ~0u || x > e.high)) e.high = x, e.index = j;
         if (x > -INFINITY) e.low = fminf(e.low, x);
     });
-    Histogram& h = a.rows[r];
-    for (uint32_t b = chunk * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
-    if (chunk == 0 && threadIdx.x == 0) h.least = 0, h.rough = 0;
     e.take_wave();
-    if (lane == 0) waves[wave] = e;
+    if ((threadIdx.x & 63u) == 0) waves[threadIdx.x >> 6] = e;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < WAVES; ++w) e.take(waves[w]);
-        a.extents[(size_t)r * a.chunks + chunk] = e;
-    }
 }
 
-// A row's extent from its chunks', and whether it is to be sampled at all.
-__device__ __forceinline__ bool row_extent(const Sample& a, uint32_t r, float temperature, Extent& e) {
-    e = Extent{-INFINITY, INFINITY, ~0u};
-    for (uint32_t c = threadIdx.x & 63u; c < a.chunks; c += 64u) e.take(a.extents[(size_t)r * a.chunks + c]);
-    e.take_wave();
+// Whether a row is to be sampled at all, and what it has if not: its highest
+// value's index, as tmh_argmax chooses it.
+__device__ __forceinline__ bool sampled(float temperature, const Extent& e) {
     return temperature > 0.0f && e.high > -INFINITY;
 }
 
-// The histogram of chunk blockIdx.y of row blockIdx.x, added to the row's.
-__global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
-    __shared__ u64 sums[BINS];
-    __shared__ double begins[BINS];
-    __shared__ uint32_t counts[BINS];
-    __shared__ u64 least_sum;
-    const uint32_t r = blockIdx.x;
-    if (r >= a.count) return;
-    const float* row = a.x + (size_t)r * a.ldx;
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-    Extent e;
-    if (!row_extent(a, r, temperature, e)) return;
-    const Measure m(e, temperature, a.shift);
-    const float least = a.min_p ? a.min_p[r] : 0.0f;
-    const uint32_t below = least <= 0.0f ? MINUS_INFINITY : m.first_below(least), border = m.bin_of_key(below);
-#pragma unroll
-    for (uint32_t i = 0; i < BINS / THREADS; ++i) {
-        const uint32_t b = threadIdx.x + i * THREADS;
-        sums[b] = 0, counts[b] = 0, begins[b] = m.begin(b);
-    }
-    if (threadIdx.x == 0) least_sum = 0;
-    __syncthreads();
-    u64 kept = 0;
-    each_value<4>(row, blockIdx.y * a.chunk, min(blockIdx.y * a.chunk + a.chunk, a.n), [&](float x, uint32_t) {
-        const float y = m.y(x);
-        if (m.within(y)) {
-            const uint32_t bin = m.bin(y);
-            const double scaled = m.scaled(x, bin, begins[bin]);
-            const u64 weight = m.whole(scaled);
-            atomicAdd(&counts[bin], 1u);
-            atomicAdd(&sums[bin], weight);
-            if (bin == border && key_of(x) < below) kept += weight;
-        }
-    });
-    if (border < BINS) {
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) kept += __shfl_xor(kept, d, 64);
-        if ((threadIdx.x & 63u) == 0) atomicAdd(&least_sum, kept);
-    }
-    __syncthreads();
-    Histogram& h = a.rows[r];
-    if (threadIdx.x == 0 && least_sum) atomicAdd(&h.least, least_sum);
-    u64 rough = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < BINS / THREADS; ++i) {
-        const uint32_t b = threadIdx.x + i * THREADS;
-        rough += scale_down(sums[b], (int)m.power(b));
-        if (a.chunks == 1u) {
-            h.counts[b] = counts[b], h.sums[b] = sums[b];
-        } else if (counts[b]) {
-            atomicAdd(&h.counts[b], counts[b]);
-            if (sums[b]) atomicAdd(&h.sums[b], sums[b]);
-        }
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) rough += __shfl_xor(rough, d, 64);
-    if ((threadIdx.x & 63u) == 0) atomicAdd(&h.rough, rough);
+__device__ __forceinline__ void take_highest(const Sample& a, uint32_t r, const Extent& e) {
+    if (threadIdx.x != 0) return;
+    const float first = a.x[(size_t)r * a.ldx];
+    a.ids[r] = first != first || e.index == ~0u ? 0 : (int32_t)e.index;
 }
 
-// One row by one workgroup: the cuts and the choice.
-__global__ __launch_bounds__(1024) void k_sample(Sample a) {
-    extern __shared__ u64 lds_words[];
-    Lds& l = *reinterpret_cast<Lds*>(lds_words);
-    const uint32_t r = blockIdx.x, n = a.n;
-    const float* row = a.x + (size_t)r * a.ldx;
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-    Extent e;
-    if (!row_extent(a, r, temperature, e)) {
-        if (threadIdx.x == 0) {
-            const float first = row[0];
-            a.ids[r] = first != first || e.index == ~0u ? 0 : (int32_t)e.index;
+// What a histogram is made in, in LDS.
+struct Counting {
+    Histogram h;
+    double begins[BINS];  // the weights at the bins' beginnings
+
+    __device__ __forceinline__ void clear(const Measure& m) {
+#pragma unroll
+        for (uint32_t i = 0; i < BINS / THREADS; ++i) {
+            const uint32_t b = threadIdx.x + i * THREADS;
+            h.sums[b] = 0, h.counts[b] = 0, begins[b] = m.begin(b);
         }
-        return;
+        if (threadIdx.x == 0) h.least = 0, h.rough = 0;
+        __syncthreads();
     }
-    const Measure m(e, temperature, a.shift);
+    // The histogram of a row or chunk.
+    __device__ __forceinline__ void count(const Measure& m, const InMemory& row, float least) {
+        const uint32_t below = least <= 0.0f ? MINUS_INFINITY : m.first_below(least), border = m.bin_of_key(below);
+        clear(m);
+        u64 kept = 0;
+        row.each<4>([&](float x, uint32_t) {
+            const float y = m.y(x);
+            if (m.within(y)) {
+                const uint32_t bin = m.bin(y);
+                const u64 weight = m.whole(m.scaled(x, bin, begins[bin]));
+                atomicAdd(&h.counts[bin], 1u);
+                atomicAdd(&h.sums[bin], weight);
+                if (bin == border && key_of(x) < below) kept += weight;
+            }
+        });
+        if (border < BINS) add(h.least, kept);
+        __syncthreads();
+        u64 rough = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < BINS / THREADS; ++i) {
+            const uint32_t b = threadIdx.x + i * THREADS;
+            rough += scale_down(h.sums[b], (int)m.power(b));
+        }
+        add(h.rough, rough);
+        __syncthreads();
+    }
+    static __device__ __forceinline__ void add(u64& to, u64 v) {
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+        if ((threadIdx.x & 63u) == 0) atomicAdd(&to, v);
+    }
+};
+
+// The cuts and the choice of row r from its histogram, by a workgroup.
+__device__ __forceinline__ void choose(const Sample& a, uint32_t r, Lds& l, const Measure& m, const InMemory& row,
+                                       const Histogram& h) {
     constexpr uint32_t PER = BINS / THREADS;
-    const Histogram& h = a.rows[r];
     // Common units of 2^-common: the sum of all weights, less than twice what it
     // roughly is, stays below 2^62 of them. A bin's own are finer by so many bits.
     const int bits = 65 - __clzll((long long)h.rough), common = 62 + (int)m.shift - bits;
@@ -660,7 +629,7 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
         if (l.found.count_before + l.found.count <= LIST) {
             // the candidates through the cut's bin: of them from here on
             listed = true;
-            list_values(l, row, n, value_of(m.first_key(l.found.bin + 1u) - 1u), m.highest);
+            list_values(l, row, value_of(m.first_key(l.found.bin + 1u) - 1u), m.highest);
             if (l.listed <= FEW) {
                 if (threadIdx.x < 64u) {
                     // in units of 2^-FINE
@@ -681,7 +650,7 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
     const auto find = [&](Target t) {
         bins.find(l, t);
         const uint32_t bin = l.found.bin;
-        find_in_bin(l, m, row, n, t, h.sums[bin], finer(bin), listed);
+        find_in_bin(l, m, row, t, h.sums[bin], finer(bin), listed);
     };
     if (cut_k) find(kth), total = l.found.sum;
     if (cut_p) find(reach((double)total)), total = min(total, l.found.sum);
@@ -689,6 +658,93 @@ __global__ __launch_bounds__(1024) void k_sample(Sample a) {
     // the highest always stays
     find(choice(max(total, scale_down((u64)1 << m.shift, (int)m.shift - common))));
     if (threadIdx.x == 0) a.ids[r] = (int32_t)l.found.index;
+}
+
+// The highest and lowest values of chunk blockIdx.y of row blockIdx.x, whose
+// share of the row's histogram it clears. Rows stand first in the grid, up to
+// a multiple of eight: a row's chunks then meet on one XCD, whose L2 holds the
+// row for the later launches.
+__global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
+    __shared__ Extent waves[WAVES];
+    const uint32_t r = blockIdx.x, chunk = blockIdx.y;
+    if (r >= a.count) return;
+    find_extent(waves, InMemory{a.x + (size_t)r * a.ldx, chunk * a.chunk, min(chunk * a.chunk + a.chunk, a.n)});
+    Histogram& h = a.rows[r];
+    for (uint32_t b = chunk * THREADS + threadIdx.x; b < BINS; b += a.chunks * THREADS) h.sums[b] = 0, h.counts[b] = 0;
+    if (threadIdx.x == 0) {
+        if (chunk == 0) h.least = 0, h.rough = 0;
+        Extent e = waves[0];
+        for (uint32_t w = 1; w < WAVES; ++w) e.take(waves[w]);
+        a.extents[(size_t)r * a.chunks + chunk] = e;
+    }
+}
+
+// A row's extent from its chunks' or its waves'.
+__device__ __forceinline__ Extent join_extents(const Extent* parts, uint32_t count) {
+    Extent e{-INFINITY, INFINITY, ~0u};
+    for (uint32_t c = threadIdx.x & 63u; c < count; c += 64u) e.take(parts[c]);
+    e.take_wave();
+    return e;
+}
+
+// The histogram of chunk blockIdx.y of row blockIdx.x, added to the row's.
+__global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
+    __shared__ Counting counting;
+    const uint32_t r = blockIdx.x, chunk = blockIdx.y;
+    if (r >= a.count) return;
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    const Extent e = join_extents(a.extents + (size_t)r * a.chunks, a.chunks);
+    if (!sampled(temperature, e)) return;
+    const Measure m(e, temperature, a.shift);
+    counting.count(m, InMemory{a.x + (size_t)r * a.ldx, chunk * a.chunk, min(chunk * a.chunk + a.chunk, a.n)},
+                   a.min_p ? a.min_p[r] : 0.0f);
+    Histogram& h = a.rows[r];
+    if (threadIdx.x == 0) {
+        atomicAdd(&h.rough, counting.h.rough);
+        if (counting.h.least) atomicAdd(&h.least, counting.h.least);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < BINS / THREADS; ++i) {
+        const uint32_t b = threadIdx.x + i * THREADS;
+        if (counting.h.counts[b]) {
+            atomicAdd(&h.counts[b], counting.h.counts[b]);
+            if (counting.h.sums[b]) atomicAdd(&h.sums[b], counting.h.sums[b]);
+        }
+    }
+}
+
+// A row from its histogram.
+__global__ __launch_bounds__(1024) void k_sample_choose(Sample a) {
+    __shared__ Lds l;
+    const uint32_t r = blockIdx.x;
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    const Extent e = join_extents(a.extents + (size_t)r * a.chunks, a.chunks);
+    if (!sampled(temperature, e)) {
+        take_highest(a, r, e);
+        return;
+    }
+    const Measure m(e, temperature, a.shift);
+    choose(a, r, l, m, InMemory{a.x + (size_t)r * a.ldx, 0, a.n}, a.rows[r]);
+}
+
+// A whole row by one workgroup: where there is a row for each compute unit or
+// nearly, chunks would gain nothing.
+__global__ __launch_bounds__(1024) void k_sample_row(Sample a) {
+    extern __shared__ u64 lds_words[];
+    Counting& counting = *reinterpret_cast<Counting*>(lds_words);
+    Lds& l = *reinterpret_cast<Lds*>(&counting + 1);
+    const uint32_t r = blockIdx.x;
+    const InMemory row{a.x + (size_t)r * a.ldx, 0, a.n};
+    find_extent(l.waves, row);
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+    const Extent e = join_extents(l.waves, WAVES);
+    if (!sampled(temperature, e)) {
+        take_highest(a, r, e);
+        return;
+    }
+    const Measure m(e, temperature, a.shift);
+    counting.count(m, row, a.min_p ? a.min_p[r] : 0.0f);
+    choose(a, r, l, m, row, counting.h);
 }
 
 int code(hipError_t e) { return e == hipErrorOutOfMemory ? TMH_ERROR_OUT_OF_MEMORY : (int)e; }
@@ -711,20 +767,27 @@ int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t tem
     if (err) return err;
     uint32_t bits = 0;
     while (n >> bits) ++bits;
+    Sample a{(const float*)x, ldx, n, std::min(62u - bits, 50u), n, 1, rows, (const float*)temperature,
+             (const int32_t*)top_k, (const float*)top_p, (const float*)min_p, (const float*)u, (int32_t*)ids, nullptr,
+             nullptr};
     // a chunk for each compute unit, of four values a thread or more
-    constexpr uint32_t LEAST = 4u * THREADS;
-    const uint32_t chunks = std::max(1u, std::min((uint32_t)ctx.compute_units / rows, (n + LEAST - 1u) / LEAST));
-    const uint32_t chunk = (n + chunks - 1u) / chunks;
-    const size_t extents = ((size_t)rows * chunks * sizeof(Extent) + 255u) & ~(size_t)255u;
-    Workspace work(ctx.index, extents + (size_t)rows * sizeof(Histogram));
-    if (work.status) return work.status;
-    Sample a{(const float*)x, ldx, n, std::min(62u - bits, 50u), chunk, (n + chunk - 1u) / chunk, rows,
-             (const float*)temperature, (const int32_t*)top_k, (const float*)top_p, (const float*)min_p,
-             (const float*)u, (int32_t*)ids, (Extent*)work.memory, (Histogram*)(work.memory + extents)};
-    const dim3 grid((rows + 7u) / 8u * 8u, a.chunks);
-    TMH_LAUNCH(k_sample_extent, grid, dim3(THREADS), 0, ctx.stream, a);
-    TMH_LAUNCH(k_sample_histogram, grid, dim3(THREADS), 0, ctx.stream, a);
-    TMH_LAUNCH(k_sample, dim3(rows), dim3(THREADS), sizeof(Lds), ctx.stream, a);
+    constexpr uint32_t LEAST = 4u * THREADS, LDS = sizeof(Counting) + sizeof(Lds);
+    const uint32_t chunks = std::min((uint32_t)ctx.compute_units / rows, (n + LEAST - 1u) / LEAST);
+    if (chunks <= 1u) {
+        TMH_LAUNCH(k_sample_row, dim3(rows), dim3(THREADS), LDS, ctx.stream, a);
+    } else {
+        a.chunk = (n + chunks - 1u) / chunks;
+        a.chunks = (n + a.chunk - 1u) / a.chunk;
+        const size_t extents = ((size_t)rows * a.chunks * sizeof(Extent) + 255u) & ~(size_t)255u;
+        Workspace work(ctx.index, extents + (size_t)rows * sizeof(Histogram));
+        if (work.status) return work.status;
+        a.extents = (Extent*)work.memory;
+        a.rows = (Histogram*)(work.memory + extents);
+        const dim3 grid((rows + 7u) / 8u * 8u, a.chunks);
+        TMH_LAUNCH(k_sample_extent, grid, dim3(THREADS), 0, ctx.stream, a);
+        TMH_LAUNCH(k_sample_histogram, grid, dim3(THREADS), 0, ctx.stream, a);
+        TMH_LAUNCH(k_sample_choose, dim3(rows), dim3(THREADS), 0, ctx.stream, a);
+    }
     const hipError_t e = hipGetLastError();
     if (e == hipSuccess) note_launch(ctx.index, 1, false);
     return code(e);

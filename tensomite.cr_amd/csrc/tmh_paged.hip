@@ -491,7 +491,9 @@ struct Few {
     static constexpr uint32_t BYTES = Split<KIND>::BYTES;
     static constexpr uint32_t CHUNKS = W * BYTES / 16u;         // 16-byte chunks of a row
     static constexpr uint32_t STAGE = 32u * W * BYTES;          // values of one step
-    static constexpr uint32_t STAGES = STAGE <= 16384u ? 2 : 1;  // ahead, where four waves' fit the LDS
+    // a step ahead, where two workgroups' then fit a compute unit's LDS and
+    // registers (48 windows of 1024, f32, 128 wide: 101 us with it, 96 without)
+    static constexpr uint32_t STAGES = STAGE <= 8192u ? 2 : 1;
     static constexpr uint32_t LOADS = STAGE / 1024u;
     static constexpr uint32_t EIGHT = BYTES / 2u;               // 16-byte pieces of eight numbers
     static constexpr uint32_t STEPS = W / 32u;                  // of the score's product
@@ -1331,16 +1333,16 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
     // Few rows: shares of the keys such that four workgroups a compute unit
     // have one each, of at least eight tiles of keys (two steps a wave; a join
     // costs more than that: 512 positions 9.0 us in two launches, 7.5 in one),
-    // or sixteen where there is a workgroup for each compute unit without (48
-    // windows of 1024: 114 -> 101 us). More rows: two a compute unit, of at least
-    // eight.
+    // or thirty-two where there is a workgroup for each compute unit without (48
+    // windows of 1024: shares of 8 tiles 97 us, whole ones 84). More rows: two a
+    // compute unit, of at least eight.
     AttendPaged few = a, more = a;
     const uint64_t rows = std::max<uint64_t>(1u, (uint64_t)max_new * group);
     few.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, rows);
     const uint32_t row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
     const uint64_t few_groups = (uint64_t)sequences * kv_heads * row_tiles;
     const uint64_t few_tiles = most_tiles(a, FEW_ROWS);
-    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, few_groups > (uint32_t)ctx.compute_units ? 16u : 8u);
+    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, few_groups > (uint32_t)ctx.compute_units ? 32u : 8u);
     const bool has_more = rows > FEW_ROWS;
     more.row_tile = width <= 64u ? 64 : 128;
     more.alone = has_more && sequences == 1u;  // one launch for the usual prompt

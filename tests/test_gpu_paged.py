@@ -470,11 +470,12 @@ def test_a_cache_past_four_gigabytes(dev, kind, width):
     row = ref.from_bits(dev.to_array(out, np.uint8, page), kind).reshape(ps, width)[place[199]]
     dev.sync()
     assert np.array_equal(row, ref.to_kind(x[-1, 3 * width:], kind)[1])
+    limit = dev.counters()["pool_limit"]
+    dev.set_pool_limit(0)  # so that the memory is given back
     for b in (big.keys, big.values):
         b.release()
-    dev.set_pool_limit(0)
-    dev.sync()  # gives the memory back
-    dev.set_pool_limit(1 << 30)
+    dev.sync()
+    dev.set_pool_limit(limit)
 
 
 def test_the_same_bits_on_every_call(dev):

@@ -179,10 +179,11 @@ def test_rows_past_four_gigabytes(dev):
     got = dev.to_array(dev.sample(big, rows, n, dev.from_array(u), ldx=ldx), np.int32, rows)
     dev.sync()
     assert list(got) == [ref.sample(x[r], u[r]) for r in range(rows)]
+    limit = dev.counters()["pool_limit"]
+    dev.set_pool_limit(0)  # so that the memory is given back
     big.release()
-    dev.set_pool_limit(0)
     dev.sync()
-    dev.set_pool_limit(1 << 30)
+    dev.set_pool_limit(limit)
 
 
 def test_lists_of_every_length(dev):

@@ -42,6 +42,11 @@ struct Paged {
     int32_t* errors;
 };
 
+// The thread's wave, in a scalar register: what follows from it stays in them.
+__device__ __forceinline__ uint32_t wave_index() {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+}
+
 struct Sequence {
     uint32_t first, count, length;  // its first row, new tokens and positions
 };
@@ -393,7 +398,6 @@ __device__ __forceinline__ void plain_rows(const AttendPaged& a, const Rows& w, 
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -514,7 +518,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float tops[4][FEW_TILE], totals[4][FEW_TILE];
     __shared__ uint32_t redo;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 15u, group = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), col = lane & 15u, group = lane >> 4;
     Rows w;
     uint32_t b = blockIdx.x;
     w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
@@ -768,9 +772,12 @@ __device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CA
 // the keys its second operand is given. F16 and BF16 tiles come by direct loads
 // into one of two buffers while the other is used; F32 ones are split in parts
 // on the way through registers, once for the four waves.
-template <uint32_t KIND, uint32_t W, uint32_t KS>
+// Rows up to 64 columns wide go 64 a workgroup, whose waves have half of the keys
+// of a step each (2048-token prompt, 32 heads of 64, f16: 53 us; 128 rows: 72).
+template <uint32_t KIND, uint32_t W>
 struct Tile {
-    static constexpr uint32_t ROWS = 128u / KS;  // query rows of a workgroup
+    static constexpr uint32_t SHARES = W <= 64u ? 2 : 1;  // of a step's keys, by wave
+    static constexpr uint32_t ROWS = 128u / SHARES;       // query rows of a workgroup
     static constexpr bool F32 = KIND == TMH_CACHE_F32;
     static constexpr uint32_t KT = W == 256u || (F32 && W == 128u) ? 32 : 64;
     static constexpr uint32_t CHUNKS = W / 8u;  // of 8 columns: 16 bytes of LDS a part
@@ -778,7 +785,6 @@ struct Tile {
     static constexpr uint32_t PARTS = Split<KIND>::CACHE_PARTS;
     static constexpr uint32_t STAGE = 2u * PARTS * PART;  // keys, then values
     static constexpr uint32_t LDS = F32 ? STAGE : 2u * STAGE;
-    static constexpr uint32_t AT_ONCE = W <= 64u && KS == 1u ? 2 : 1;  // scores of so many times 32 keys before their softmax
     static constexpr uint32_t LOADS = KT * CHUNKS / 256u;  // chunks a thread brings of keys, and of values
     static __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t chunk, uint32_t row) {
         return chunk ^ (row & (CHUNKS - 1u) & 7u);
@@ -815,14 +821,14 @@ __device__ __forceinline__ bool find_row_tile(const AttendPaged& a, uint32_t til
     return false;
 }
 
-template <uint32_t KIND, uint32_t W, uint32_t KS>
+template <uint32_t KIND, uint32_t W>
 __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
-    typedef Tile<KIND, W, KS> T;
-    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT;
+    typedef Tile<KIND, W> T;
+    constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT, SHARES = T::SHARES;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ uint32_t redo[T::ROWS / 32u], cache_rows[2][KT];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = lane & 31u, half = lane >> 5;
-    const uint32_t rows_of = wave % (4u / KS), keys_of = wave / (4u / KS);  // the wave's 32 rows, its share of the keys
+    const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), col = lane & 31u, half = lane >> 5;
+    const uint32_t rows_of = wave % (4u / SHARES), keys_of = wave / (4u / SHARES);  // the wave's 32 rows, its share of the keys
     Rows w;
     uint32_t b = blockIdx.x;
     w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
@@ -958,88 +964,84 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
         if (looks) ahead = w.cache_row_for(a, first_key(i + 2u) + lane % KT);
         const uint32_t k0 = first_key(i);
 #pragma unroll
-        for (uint32_t g1 = 0; g1 < KT / 32u; g1 += T::AT_ONCE * KS) {
-            const uint32_t g0 = g1 + keys_of, kg0 = k0 + g0 * 32u;
+        for (uint32_t g0 = 0; g0 < KT / 32u; g0 += SHARES) {
+            const uint32_t g = g0 + keys_of, kg = k0 + g * 32u;
             // keys that none of the wave's rows sees
-            if (idle || kg0 > hi || (kg0 >= a.sinks && kg0 + T::AT_ONCE * 32u <= window_start(a, lo))) continue;
-            f32x16 scores[T::AT_ONCE];
+            if (idle || kg > hi || (kg >= a.sinks && kg + 32u <= window_start(a, lo))) continue;
+            // ahead of other waves' vector operations (512 tokens at the end of 30000,
+            // bf16, 128 wide: 612 us, 596 with it)
+            __builtin_amdgcn_s_setprio(1);
+            f32x16 score = f32x16{} * 0.0f;
 #pragma unroll
-            for (uint32_t g = 0; g < T::AT_ONCE; ++g) {
-                scores[g] = f32x16{} * 0.0f;
+            for (uint32_t k = 0; k < W / 16u; ++k) {
+                Operand<CP> o;
+                const uint32_t row = g * 32u + col;
 #pragma unroll
-                for (uint32_t k = 0; k < W / 16u; ++k) {
+                for (uint32_t p = 0; p < CP; ++p)
+                    o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
+                score = multiply_parts32<KIND>(o, query[k], score);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
+            if (!whole) {
+#pragma unroll
+                for (uint32_t j = 0; j < 16u; ++j)
+                    if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
+            }
+            float best = score[0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
+            if (__any(best > limit)) {
+                best = fmaxf(best, __shfl_xor(best, 32, 64));
+                if (best > limit) {
+                    const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((zero - best) * undo + HEADROOM);
+                    zero = best - HEADROOM * power;
+                    limit = best + SLACK * power;
+                    total *= keep;
+#pragma unroll
+                    for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
+                }
+            }
+            score -= zero;
+            if (KIND == TMH_CACHE_F16 && scaled) {
+                asm volatile("");  // a branch: most rows have no power
+#pragma unroll
+                for (int j = 0; j < 16; ++j) score[j] *= undo;
+            }
+            Operand<NP> weight[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
+                sum += e0;
+                sum += e1;
+                split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
+            }
+            total += sum;
+#pragma unroll
+            for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+                for (uint32_t c = 0; c < 2u; ++c) {
+                    // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
                     Operand<CP> o;
-                    const uint32_t row = (g0 + g) * 32u + col;
+                    const uint32_t row = g * 32u + c * 16u + half * 4u + col % 16u / 4u;
+                    const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
 #pragma unroll
-                    for (uint32_t p = 0; p < CP; ++p)
-                        o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
-                    scores[g] = multiply_parts32<KIND>(o, query[k], scores[g]);
-                }
-            }
-#pragma unroll
-            for (uint32_t g = 0; g < T::AT_ONCE; ++g) {
-                f32x16& score = scores[g];
-                const uint32_t kg = kg0 + g * 32u;
-                const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
-                if (!whole) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 16u; ++j)
-                        if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
-                }
-                float best = score[0];
-#pragma unroll
-                for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
-                if (__any(best > limit)) {
-                    best = fmaxf(best, __shfl_xor(best, 32, 64));
-                    if (best > limit) {
-                        const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((zero - best) * undo + HEADROOM);
-                        zero = best - HEADROOM * power;
-                        limit = best + SLACK * power;
-                        total *= keep;
-#pragma unroll
-                        for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
+                    for (uint32_t p = 0; p < CP; ++p) {
+                        const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
+                        const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
+                        const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
+                        o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
                     }
+                    out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
                 }
-                score -= zero;
-                if (KIND == TMH_CACHE_F16 && scaled) {
-                    asm volatile("");  // a branch: most rows have no power
-                    score *= undo;
-                }
-                Operand<NP> weight[2];
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
-                    sum += e0;
-                    sum += e1;
-                    split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
-                }
-                total += sum;
-#pragma unroll
-                for (uint32_t d = 0; d < W / 32u; ++d)
-#pragma unroll
-                    for (uint32_t c = 0; c < 2u; ++c) {
-                        // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
-                        Operand<CP> o;
-                        const uint32_t row = (g0 + g) * 32u + c * 16u + half * 4u + col % 16u / 4u;
-                        const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
-#pragma unroll
-                        for (uint32_t p = 0; p < CP; ++p) {
-                            const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
-                            const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
-                            const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
-                            o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
-                        }
-                        out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
-                    }
-            }
         }
         if (looks && lane < KT) cache_rows[i & 1u][lane] = ahead;
     }
 
     total += __shfl_xor(total, 32, 64);
     float top = limit == -INFINITY ? -INFINITY : zero * undo;
-    if constexpr (KS == 2u) {
+    if constexpr (SHARES == 2u) {
         // the rows' other half of the keys
         float* other = (float*)lds + (rows_of * 64u + lane) * (W / 2u + 4u);
         lds_sync();
@@ -1202,22 +1204,22 @@ void launch_few_of(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipS
         launch_few<KIND, 256>(a, row_tiles, grid, stream);
 }
 
-template <uint32_t KIND, uint32_t W, uint32_t KS>
+template <uint32_t KIND, uint32_t W>
 void launch_tile(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
-    constexpr uint32_t lds = Tile<KIND, W, KS>::LDS;
-    TMH_LAUNCH((k_attend_tile<KIND, W, KS>), dim3(grid), dim3(256), lds, stream, a);
+    constexpr uint32_t lds = Tile<KIND, W>::LDS;
+    TMH_LAUNCH((k_attend_tile<KIND, W>), dim3(grid), dim3(256), lds, stream, a);
 }
 
 template <uint32_t KIND>
 void launch_tile_of(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
     if (a.p.width <= 32u)
-        a.row_tile == 128u ? launch_tile<KIND, 32, 1>(a, grid, stream) : launch_tile<KIND, 32, 2>(a, grid, stream);
+        launch_tile<KIND, 32>(a, grid, stream);
     else if (a.p.width <= 64u)
-        a.row_tile == 128u ? launch_tile<KIND, 64, 1>(a, grid, stream) : launch_tile<KIND, 64, 2>(a, grid, stream);
+        launch_tile<KIND, 64>(a, grid, stream);
     else if (a.p.width <= 128u)
-        launch_tile<KIND, 128, 1>(a, grid, stream);
+        launch_tile<KIND, 128>(a, grid, stream);
     else
-        launch_tile<KIND, 256, 1>(a, grid, stream);
+        launch_tile<KIND, 256>(a, grid, stream);
 }
 
 // Tiles of keys that a row tile of `tokens` new tokens sees, at most.

@@ -424,8 +424,8 @@ int tmh_argmax(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t ids
  * they were; a page out of range is not read or written, and the rows that
  * see it are unspecified. Both are index errors, reported at tmh_sync.
  * `kind` is the cache's element type (ggml's numbering, as tmh_gguf_tensor's);
- * keys and values are 16-byte aligned, width a multiple of 8 up to 256, and
- * pages * kv_heads * page_size below 2^31. */
+ * keys and values are 16-byte aligned, width a multiple of 8 up to 256, tokens
+ * below 2^24 and pages * kv_heads * page_size below 2^31. */
 #define TMH_CACHE_F32 0
 #define TMH_CACHE_F16 1
 #define TMH_CACHE_BF16 30
@@ -446,9 +446,11 @@ int tmh_rope_write_paged(uint64_t x, uint32_t ldx, uint32_t tokens, uint32_t hea
  * or j < sinks (the first `sinks` positions stay visible); window 0 is no
  * window. What hidden positions hold, NaN and infinity included, does not
  * reach a result. Query head h reads kv head h / (heads / kv_heads); q rows
- * are `ldq` apart ([heads, width] each), dst rows `ld_dst` apart, both F32.
- * No sequence may have more than `max_new` new tokens or `max_length`
- * positions (they size the launch). */
+ * are `ldq` apart ([heads, width] each), dst rows `ld_dst` apart, both F32; q
+ * and dst may not overlap. No sequence may have more than `max_new` new tokens
+ * or `max_length` positions: they size the launch, which is the fastest where
+ * they are the batch's own. A launch of 2^24 workgroups or more (a workgroup is
+ * 16 rows of a kv head, or 64) is a shape error. */
 int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t heads, uint32_t kind, uint64_t keys,
                         uint64_t values, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t width,
                         uint64_t page_table, uint32_t table_width, uint32_t sequences, uint64_t starts,
@@ -465,8 +467,8 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
  * passes u[r] (f32 in [0, 1)) times the sum of what stayed. temperature[r]
  * not above 0 is tmh_argmax. temperature, top_k, top_p and min_p may each be 0
  * (no array): 1, all, 1 and 0. Sums and the weights are in 64 bits: the same
- * inputs give the same ids on every call. NaN is never chosen while another
- * candidate is there; n is at most 2^24, rows 65535. */
+ * inputs give the same ids on every call. Of a sampled row NaN is never chosen
+ * while another candidate above -inf is there; n is at most 2^24, rows 65535. */
 int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t temperature, uint64_t top_k,
                uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids);
 

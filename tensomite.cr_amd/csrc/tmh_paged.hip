@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256) void k_rope_write_paged(WritePaged a) {
     const uint32_t i = t - q.first;
     const uint32_t pos = q.length - q.count + i;
     if (!fits || i >= q.count || pos >= a.table_rows) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) report(a.p.errors, (int32_t)(fits ? pos : s), (int32_t)(fits ? a.table_rows : a.p.sequences));
+        if (threadIdx.x == 0 && blockIdx.y == 0)
+            report(a.p.errors, (int32_t)(fits ? pos : s), (int32_t)(fits ? a.table_rows : a.p.sequences));
         return;
     }
     const uint32_t width = a.p.width, half = width >> 1, per = width >> 3;
@@ -215,6 +216,7 @@ struct AttendPaged {
 constexpr uint32_t KEYS = 64;      // positions of a tile of keys
 constexpr uint32_t FEW_TILE = 16;  // query rows of a tile of few rows
 constexpr uint32_t FEW_ROWS = 32;  // the most query rows of a kv head that are few
+constexpr uint32_t MOST_GROUPS = (1u << 24) - 1u;  // workgroups of 256 threads that a launch can have
 
 // The tiles of keys that positions [lo, hi] see: `early` of the sinks, then
 // those from the window's first, `from`, on.
@@ -512,15 +514,14 @@ struct Few {
 };
 
 template <uint32_t KIND, uint32_t W>
-__global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_tiles) {
+__device__ __forceinline__ void attend_few(const AttendPaged& a, uint32_t row_tiles, uint32_t block, uint8_t* lds) {
     typedef Few<KIND, W> F;
     constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float tops[4][FEW_TILE], totals[4][FEW_TILE];
     __shared__ uint32_t redo;
     const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), col = lane & 15u, group = lane >> 4;
     Rows w;
-    uint32_t b = blockIdx.x;
+    uint32_t b = block;
     w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
     const uint32_t row_tile = b % row_tiles;
     b /= row_tiles;
@@ -738,6 +739,12 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_
     if (again) plain_rows<KIND>(a, w, part, &again);
 }
 
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_few(AttendPaged a, uint32_t row_tiles) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    attend_few<KIND, W>(a, row_tiles, blockIdx.x, lds);
+}
+
 // --------------------------------------------------------------- more query rows
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -822,19 +829,18 @@ __device__ __forceinline__ bool find_row_tile(const AttendPaged& a, uint32_t til
 }
 
 template <uint32_t KIND, uint32_t W>
-__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
+__device__ __forceinline__ void attend_tile(const AttendPaged& a, uint32_t block, uint8_t* lds) {
     typedef Tile<KIND, W> T;
     constexpr uint32_t CP = Split<KIND>::CACHE_PARTS, NP = Split<KIND>::PARTS, KT = T::KT, SHARES = T::SHARES;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ uint32_t redo[T::ROWS / 32u], cache_rows[2][KT];
     const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), col = lane & 31u, half = lane >> 5;
     const uint32_t rows_of = wave % (4u / SHARES), keys_of = wave / (4u / SHARES);  // the wave's 32 rows, its share of the keys
     Rows w;
-    uint32_t b = blockIdx.x;
+    uint32_t b = block;
     w.kh = b % a.p.kv_heads, b /= a.p.kv_heads;
     const uint32_t part = b % a.splits;
     if (!find_row_tile(a, b / a.splits, part, w)) {
-        if (a.alone && blockIdx.x == 0 && threadIdx.x == 0 && !read_sequence(a.p, 0, w.sq)) report(a.p.errors, 0, 1);
+        if (a.alone && block == 0 && threadIdx.x == 0 && !read_sequence(a.p, 0, w.sq)) report(a.p.errors, 0, 1);
         return;
     }
     const uint32_t width = a.p.width;
@@ -1101,6 +1107,26 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
     if (any) plain_rows<KIND>(a, w, part, redo);
 }
 
+// One sequence, of more rows than few.
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    attend_tile<KIND, W>(a, blockIdx.x, lds);
+}
+
+// A batch with sequences of both kinds: row tiles in the first `tiles`
+// workgroups, few rows behind them, so that each fills what the other leaves
+// (chunks and decode steps of 12 sequences, f32, 9 heads of 64: two launches in
+// turn 36.5 us, 25.1 so).
+template <uint32_t KIND, uint32_t W>
+__global__ __launch_bounds__(256) void k_attend_mixed(AttendPaged more, AttendPaged few, uint32_t tiles, uint32_t row_tiles) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    if (blockIdx.x < tiles)
+        attend_tile<KIND, W>(more, blockIdx.x, lds);
+    else
+        attend_few<KIND, W>(few, row_tiles, blockIdx.x - tiles, lds);
+}
+
 // Joins the parts of row r, by a wave: each part brought to the highest reference
 // and added. The parts wait in L2 or memory, so latency bounds it: a load takes
 // 64 / (width / 4) parts, and eight loads go out before the first is used.
@@ -1159,67 +1185,66 @@ __device__ __forceinline__ void join_row(const AttendPaged& a, const Rows& w, ui
     }
 }
 
-// Joins few rows, a wave a row, by sequence, kv head and row.
-__global__ __launch_bounds__(256) void k_attend_join_few(AttendPaged a, uint32_t count) {
+// Joins the rows that came in parts: a quarter of a row tile, a quarter of that a
+// wave, in the first 4 `groups` workgroups; then few rows, a wave a row, by
+// sequence, kv head and row, `count` of them.
+__global__ __launch_bounds__(256) void k_attend_join(AttendPaged more, AttendPaged few, uint32_t groups, uint32_t count) {
     __shared__ f32x4 lanes[4][64];
-    uint32_t b = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const uint32_t wave = wave_index();
+    Rows w;
+    if (blockIdx.x < 4u * groups) {
+        const uint32_t b = blockIdx.x / 4u, quarter = blockIdx.x % 4u;
+        w.kh = b % more.p.kv_heads;
+        if (!find_row_tile(more, b / more.p.kv_heads, 0, w) || w.parts == 1u) return;
+        const uint32_t from = quarter * (more.row_tile / 4u) + wave * (more.row_tile / 16u);
+        for (uint32_t i = from; i < min(from + more.row_tile / 16u, w.count); ++i) join_row(more, w, w.first + i, lanes[wave]);
+        return;
+    }
+    uint32_t b = (blockIdx.x - 4u * groups) * 4u + wave;
     if (b >= count) return;
-    Rows w;
-    const uint32_t r = b % a.room;
-    b /= a.room;
-    w.kh = b % a.p.kv_heads;
-    w.s = b / a.p.kv_heads;
-    if (!read_sequence(a.p, w.s, w.sq)) return;
-    const uint32_t rows = w.sq.count * a.group.d;
-    if (rows > FEW_ROWS || r >= rows || !w.set(a, r / FEW_TILE * FEW_TILE, FEW_TILE, 0) || w.parts == 1u) return;
-    join_row(a, w, r, lanes[threadIdx.x >> 6]);
+    const uint32_t r = b % few.room;
+    b /= few.room;
+    w.kh = b % few.p.kv_heads;
+    w.s = b / few.p.kv_heads;
+    if (!read_sequence(few.p, w.s, w.sq)) return;
+    const uint32_t rows = w.sq.count * few.group.d;
+    if (rows > FEW_ROWS || r >= rows || !w.set(few, r / FEW_TILE * FEW_TILE, FEW_TILE, 0) || w.parts == 1u) return;
+    join_row(few, w, r, lanes[wave]);
 }
 
-// Joins a quarter of a row tile, a quarter of that a wave.
-__global__ __launch_bounds__(256) void k_attend_join_tile(AttendPaged a) {
-    __shared__ f32x4 lanes[4][64];
-    Rows w;
-    w.kh = blockIdx.x % a.p.kv_heads;
-    if (!find_row_tile(a, blockIdx.x / a.p.kv_heads, 0, w) || w.parts == 1u) return;
-    const uint32_t from = blockIdx.y * (a.row_tile / 4u) + (threadIdx.x >> 6) * (a.row_tile / 16u);
-    for (uint32_t i = from; i < min(from + a.row_tile / 16u, w.count); ++i)
-        join_row(a, w, w.first + i, lanes[threadIdx.x >> 6]);
-}
+// A call's launches: `few` and `more` are its sequences of few rows and of more.
+struct Launch {
+    AttendPaged few, more;
+    uint32_t row_tiles;               // of few rows, the most of a sequence and kv head
+    uint32_t few_groups, more_groups;  // row tiles times kv heads; 0 where there are none
+    hipStream_t stream;
+};
 
 template <uint32_t KIND, uint32_t W>
-void launch_few(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipStream_t stream) {
-    constexpr uint32_t lds = Few<KIND, W>::LDS;
-    TMH_LAUNCH((k_attend_few<KIND, W>), dim3(grid), dim3(256), lds, stream, a, row_tiles);
+void launch_width(const Launch& l) {
+    constexpr uint32_t lds_few = Few<KIND, W>::LDS, lds_more = Tile<KIND, W>::LDS;
+    const uint32_t few = l.few_groups * l.few.splits, more = l.more_groups * l.more.splits;
+    if (!more) {
+        TMH_LAUNCH((k_attend_few<KIND, W>), dim3(few), dim3(256), lds_few, l.stream, l.few, l.row_tiles);
+    } else if (!few) {
+        TMH_LAUNCH((k_attend_tile<KIND, W>), dim3(more), dim3(256), lds_more, l.stream, l.more);
+    } else {
+        TMH_LAUNCH((k_attend_mixed<KIND, W>), dim3(more + few), dim3(256), std::max(lds_few, lds_more), l.stream, l.more,
+                   l.few, more, l.row_tiles);
+    }
 }
 
 template <uint32_t KIND>
-void launch_few_of(const AttendPaged& a, uint32_t row_tiles, uint32_t grid, hipStream_t stream) {
-    if (a.p.width <= 32u)
-        launch_few<KIND, 32>(a, row_tiles, grid, stream);
-    else if (a.p.width <= 64u)
-        launch_few<KIND, 64>(a, row_tiles, grid, stream);
-    else if (a.p.width <= 128u)
-        launch_few<KIND, 128>(a, row_tiles, grid, stream);
+void launch_attention_paged(const Launch& l) {
+    const uint32_t width = l.few.p.width;
+    if (width <= 32u)
+        launch_width<KIND, 32>(l);
+    else if (width <= 64u)
+        launch_width<KIND, 64>(l);
+    else if (width <= 128u)
+        launch_width<KIND, 128>(l);
     else
-        launch_few<KIND, 256>(a, row_tiles, grid, stream);
-}
-
-template <uint32_t KIND, uint32_t W>
-void launch_tile(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
-    constexpr uint32_t lds = Tile<KIND, W>::LDS;
-    TMH_LAUNCH((k_attend_tile<KIND, W>), dim3(grid), dim3(256), lds, stream, a);
-}
-
-template <uint32_t KIND>
-void launch_tile_of(const AttendPaged& a, uint32_t grid, hipStream_t stream) {
-    if (a.p.width <= 32u)
-        launch_tile<KIND, 32>(a, grid, stream);
-    else if (a.p.width <= 64u)
-        launch_tile<KIND, 64>(a, grid, stream);
-    else if (a.p.width <= 128u)
-        launch_tile<KIND, 128>(a, grid, stream);
-    else
-        launch_tile<KIND, 256>(a, grid, stream);
+        launch_width<KIND, 256>(l);
 }
 
 // Tiles of keys that a row tile of `tokens` new tokens sees, at most.
@@ -1230,33 +1255,11 @@ uint64_t most_tiles(const AttendPaged& a, uint32_t tokens) {
 }
 
 // Shares of the keys for `groups` row tiles of at most `tiles` tiles of keys:
-// so that there are `wanted` workgroups, of at least `least` tiles each.
+// so that there are at most `wanted` workgroups, or one a row tile, of at least
+// `least` tiles each.
 void set_shares(AttendPaged& a, uint64_t groups, uint64_t tiles, uint64_t wanted, uint32_t least) {
-    a.share = (uint32_t)std::max<uint64_t>(least, groups * tiles / wanted);
+    a.share = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(least, (groups * tiles + wanted - 1u) / wanted), 0x7fffffffu);
     a.splits = (uint32_t)std::max<uint64_t>(1u, (tiles + a.share - 1u) / a.share);
-}
-
-template <uint32_t KIND>
-hipError_t launch_attention_paged(const AttendPaged& few, uint32_t few_groups, uint32_t row_tiles,
-                                  const AttendPaged& more, uint32_t more_groups, hipStream_t stream) {
-    hipError_t e = hipSuccess;
-    if (more_groups) {
-        launch_tile_of<KIND>(more, more_groups * more.splits, stream);
-        e = hipGetLastError();
-        if (e == hipSuccess && more.splits > 1u) {
-            TMH_LAUNCH(k_attend_join_tile, dim3(more_groups, 4), dim3(256), 0, stream, more);
-            e = hipGetLastError();
-        }
-    }
-    if (e != hipSuccess || more.alone) return e;
-    launch_few_of<KIND>(few, row_tiles, few_groups * few.splits, stream);
-    e = hipGetLastError();
-    if (e == hipSuccess && few.splits > 1u) {
-        const uint32_t rows = few.p.sequences * few.p.kv_heads * few.room;
-        TMH_LAUNCH(k_attend_join_few, dim3((rows + 3u) / 4u), dim3(256), 0, stream, few, rows);
-        e = hipGetLastError();
-    }
-    return e;
 }
 
 int check_paged(uint32_t tokens, uint32_t kind, uint32_t pages, uint32_t page_size, uint32_t kv_heads, uint32_t width,
@@ -1264,7 +1267,7 @@ int check_paged(uint32_t tokens, uint32_t kind, uint32_t pages, uint32_t page_si
     if (kind != TMH_CACHE_F32 && kind != TMH_CACHE_F16 && kind != TMH_CACHE_BF16) return TMH_ERROR_DTYPE;
     if (width == 0 || width % 8u != 0 || width > 256u || kv_heads == 0 || kv_heads > 65535u) return TMH_ERROR_SHAPE;
     if (pages == 0 || page_size == 0 || table_width == 0) return TMH_ERROR_SHAPE;
-    if (tokens > 0x7fffffffu || sequences > 0x7ffffffeu || (uint64_t)sequences * table_width > 0x7fffffffull ||
+    if (tokens > MOST_GROUPS || sequences > 0x7ffffffeu || (uint64_t)sequences * table_width > 0x7fffffffull ||
         (uint64_t)pages * kv_heads > 0x7fffffffull || (uint64_t)pages * kv_heads * page_size > 0x7fffffffull)
         return TMH_ERROR_SHAPE;
     return TMH_SUCCESS;
@@ -1332,27 +1335,34 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
                    tokens, max_new, max_length, pages, kv_heads, width, Divider(page_size), ctx.errors},
                   (const float*)q, ldq, heads, Divider(group), (const void*)keys, (const void*)values, window, sinks,
                   (float)((double)scale * 1.4426950408889634), (float*)dst, ld_dst, 0, 1, 0, 128, 0, nullptr, nullptr};
-    // Few rows: shares of the keys such that four workgroups a compute unit
-    // have one each, of at least eight tiles of keys (two steps a wave; a join
-    // costs more than that: 512 positions 9.0 us in two launches, 7.5 in one),
-    // or thirty-two where there is a workgroup for each compute unit without (48
-    // windows of 1024: shares of 8 tiles 97 us, whole ones 84). More rows: two a
-    // compute unit, of at least eight.
-    AttendPaged few = a, more = a;
+    Launch l{a, a, 0, 0, 0, ctx.stream};
+    AttendPaged &few = l.few, &more = l.more;
     const uint64_t rows = std::max<uint64_t>(1u, (uint64_t)max_new * group);
-    few.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, rows);
-    const uint32_t row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
-    const uint64_t few_groups = (uint64_t)sequences * kv_heads * row_tiles;
-    const uint64_t few_tiles = most_tiles(a, FEW_ROWS);
-    set_shares(few, few_groups, few_tiles, 4u * ctx.compute_units, few_groups > (uint32_t)ctx.compute_units ? 32u : 8u);
     const bool has_more = rows > FEW_ROWS;
     more.row_tile = width <= 64u ? 64 : 128;
-    more.alone = has_more && sequences == 1u;  // one launch for the usual prompt
-    // row tiles of all sequences, at most
-    const uint64_t more_groups =
-        ((uint64_t)tokens * group / more.row_tile + std::min<uint64_t>(sequences, more.alone ? 1u : (uint64_t)tokens * group / (FEW_ROWS + 1u))) * kv_heads;
-    if (has_more) set_shares(more, more_groups, most_tiles(a, more.row_tile), 2u * ctx.compute_units, 8u);
-    if (few_groups * few.splits > 0x7fffffffull || more_groups * more.splits > 0x7fffffffull) return TMH_ERROR_SHAPE;
+    more.alone = has_more && sequences == 1u;  // the usual prompt
+    few.room = (uint32_t)std::min<uint64_t>(FEW_ROWS, rows);
+    l.row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
+    uint64_t few_groups = 0, more_groups = 0;
+    if (!more.alone) {
+        // four workgroups a compute unit, a share of at least eight tiles of keys
+        // (two steps a wave; a join costs more than that: 512 positions 9.0 us in
+        // two launches, 7.5 in one), or thirty-two where row tiles alone are more
+        // than compute units (48 windows of 1024: shares of 8 tiles 97 us, whole 84)
+        few_groups = (uint64_t)sequences * kv_heads * l.row_tiles;
+        set_shares(few, few_groups, most_tiles(a, FEW_ROWS), 4u * ctx.compute_units,
+                   few_groups > (uint32_t)ctx.compute_units ? 32u : 8u);
+    }
+    if (has_more) {
+        // row tiles of all sequences, at most; two workgroups a compute unit
+        const uint64_t all = (uint64_t)tokens * group;
+        more_groups = (all / more.row_tile + std::min<uint64_t>(sequences, all / (FEW_ROWS + 1u))) * kv_heads;
+        if (more.alone) more_groups = (all + more.row_tile - 1u) / more.row_tile * kv_heads;
+        set_shares(more, more_groups, most_tiles(a, more.row_tile), 2u * ctx.compute_units, 8u);
+    }
+    if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / 8u)
+        return TMH_ERROR_SHAPE;
+    l.few_groups = (uint32_t)few_groups, l.more_groups = (uint32_t)more_groups;
     const size_t few_parts = few.splits > 1u ? (size_t)sequences * kv_heads * few.room * few.splits : 0;
     const size_t more_parts = more.splits > 1u ? (size_t)tokens * heads * more.splits : 0;
     const size_t sums = ((few_parts + more_parts) * sizeof(float2) + 255u) & ~(size_t)255u;
@@ -1362,13 +1372,18 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
     few.part = (float*)(work.memory + sums);
     more.part_sums = few.part_sums + few_parts;
     more.part = few.part + few_parts * width;
-    hipError_t e;
     if (kind == TMH_CACHE_F32)
-        e = launch_attention_paged<TMH_CACHE_F32>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
+        launch_attention_paged<TMH_CACHE_F32>(l);
     else if (kind == TMH_CACHE_F16)
-        e = launch_attention_paged<TMH_CACHE_F16>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
+        launch_attention_paged<TMH_CACHE_F16>(l);
     else
-        e = launch_attention_paged<TMH_CACHE_BF16>(few, (uint32_t)few_groups, row_tiles, more, has_more ? (uint32_t)more_groups : 0u, ctx.stream);
+        launch_attention_paged<TMH_CACHE_BF16>(l);
+    hipError_t e = hipGetLastError();
+    const uint32_t groups = more_parts ? l.more_groups : 0u, count = few_parts ? sequences * kv_heads * few.room : 0u;
+    if (e == hipSuccess && (groups || count)) {
+        TMH_LAUNCH(k_attend_join, dim3(4u * groups + (count + 3u) / 4u), dim3(256), 0, ctx.stream, more, few, groups, count);
+        e = hipGetLastError();
+    }
     if (e == hipSuccess) note_launch(ctx.index, 1, true);
     return code(e);
 }

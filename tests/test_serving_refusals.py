@@ -31,7 +31,8 @@ def sample(x=P, ldx=100, rows=3, n=100, t=P, k=P, p=P, m=P, u=P, ids=P):
 SHAPE, VALUE, DTYPE = th.ERROR_SHAPE, th.ERROR_INVALID_VALUE, th.ERROR_DTYPE
 CACHE = [(dict(kind=2), DTYPE), (dict(kind=8), DTYPE), (dict(width=0), SHAPE), (dict(width=12), SHAPE),
          (dict(width=264), SHAPE), (dict(kv=0), SHAPE), (dict(pages=0), SHAPE), (dict(page_size=0), SHAPE),
-         (dict(table_width=0), SHAPE), (dict(pages=1 << 20, page_size=1 << 10), SHAPE), (dict(tokens=1 << 31), SHAPE),
+         (dict(table_width=0), SHAPE), (dict(pages=1 << 20, page_size=1 << 10), SHAPE), (dict(tokens=1 << 24), SHAPE),
+         (dict(tokens=1 << 31), SHAPE),
          (dict(sequences=1 << 16, table_width=1 << 15), SHAPE), (dict(keys=0), VALUE), (dict(values=0), VALUE),
          (dict(keys=P + 8), VALUE), (dict(values=P + 2), VALUE), (dict(table=0), VALUE), (dict(starts=0), VALUE),
          (dict(lengths=0), VALUE)]

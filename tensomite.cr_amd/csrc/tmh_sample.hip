@@ -41,6 +41,18 @@ constexpr uint32_t LIST = 4096;  // candidates held in LDS
 constexpr uint32_t FEW = 64;     // of which so many are put in order, one a lane
 constexpr uint32_t FIRST = 512;  // a chunk's first candidates, for the row's list
 
+// v of the lane `CTRL` says, 0 where there is none or the row is not in MASK.
+template <int CTRL, int MASK>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, MASK, 0xF, true);
+}
+
+// v of the lane n before this one among its sixteen, in a ring.
+template <int N>
+__device__ __forceinline__ uint32_t ring(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x120 + N, 0xF, 0xF, false);
+}
+
 // A chunk's highest value that is a number and its first index (or ~0), and
 // its lowest value but -inf.
 struct Extent {
@@ -51,9 +63,25 @@ struct Extent {
         if (o.index != ~0u && (index == ~0u || o.high > high || (o.high == high && o.index < index)))
             high = o.high, index = o.index;
     }
+    template <int N>
+    __device__ __forceinline__ void take_ring() {
+        Extent o;
+        o.high = __uint_as_float(ring<N>(__float_as_uint(high)));
+        o.low = __uint_as_float(ring<N>(__float_as_uint(low)));
+        o.index = ring<N>(index);
+        take(o);
+    }
+    // every sixteen lanes'
+    __device__ __forceinline__ void take_sixteen() {
+        take_ring<8>();
+        take_ring<4>();
+        take_ring<2>();
+        take_ring<1>();
+    }
     __device__ __forceinline__ void take_wave() {
+        take_sixteen();
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
+        for (int d = 16; d <= 32; d <<= 1) {
             Extent o;
             o.high = __shfl_xor(high, d, 64);
             o.low = __shfl_xor(low, d, 64);
@@ -164,7 +192,7 @@ struct Measure {
 
     __device__ __forceinline__ Measure(const Extent& e, float temperature, uint32_t bits) {
         constexpr float MOST = 3.4028234663852886e38f;
-        exact = uniform(1.4426950408889634 / (double)fmaxf(temperature, 1e-38f));
+        exact = uniform(1.4426950408889634 / (double)fminf(fmaxf(temperature, 1e-38f), MOST));
         scale = uniform((float)exact);
         const float span = (e.high - e.low) * scale;  // infinite or none where the highest is infinite
         const float end = span <= 80.0f ? span : 80.0f;
@@ -274,7 +302,8 @@ struct Lds {
     u64 zoom_sums[ZOOM];
     u64 list[LIST];  // key, then index
     u64 few[FEW];    // those of them the target is among
-    u64 weights[FEW];
+    u64 weights[FEW], sums_before[FEW];
+    uint32_t counts_before[FEW];
     uint32_t zoom_counts[ZOOM];
     u64 wave_sum[WAVES];
     uint32_t wave_count[WAVES];
@@ -284,17 +313,21 @@ struct Lds {
     uint32_t keys[2];  // the first of a bin, and of the next
 };
 
-// v of the lane `CTRL` says, 0 where there is none or the row is not in MASK.
-template <int CTRL, int MASK>
-__device__ __forceinline__ uint32_t dpp(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, MASK, 0xF, true);
-}
-
 // One step of the wave's running sums.
 template <int CTRL, int MASK>
 __device__ __forceinline__ void scan_step(uint32_t& c, u64& s) {
     c += dpp<CTRL, MASK>(c);
     s += (u64)dpp<CTRL, MASK>((uint32_t)(s >> 32)) << 32 | dpp<CTRL, MASK>((uint32_t)s);
+}
+
+// Running sums of the wave's lanes.
+__device__ __forceinline__ void scan_wave(uint32_t& c, u64& s) {
+    scan_step<0x111, 0xF>(c, s);  // 1, 2, 4 and 8 lanes back within each 16
+    scan_step<0x112, 0xF>(c, s);
+    scan_step<0x114, 0xF>(c, s);
+    scan_step<0x118, 0xF>(c, s);
+    scan_step<0x142, 0xA>(c, s);  // lane 15's to the next 16, lane 31's to the upper half
+    scan_step<0x143, 0xC>(c, s);
 }
 
 // Replaces count and sum by what the threads before this one hold of them;
@@ -303,12 +336,7 @@ __device__ __forceinline__ void scan(u64* wave_sum, uint32_t* wave_count, uint32
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     uint32_t c = count;
     u64 s = sum;
-    scan_step<0x111, 0xF>(c, s);  // 1, 2, 4 and 8 lanes back within each 16
-    scan_step<0x112, 0xF>(c, s);
-    scan_step<0x114, 0xF>(c, s);
-    scan_step<0x118, 0xF>(c, s);
-    scan_step<0x142, 0xA>(c, s);  // lane 15's to the next 16, lane 31's to the upper half
-    scan_step<0x143, 0xC>(c, s);
+    scan_wave(c, s);
     __syncthreads();
     if (lane == 63u) wave_count[wave] = c, wave_sum[wave] = s;
     __syncthreads();
@@ -441,12 +469,8 @@ __device__ __forceinline__ void list_values(Lds& l, const InMemory& row, float l
         if (!__any(mine != 0)) continue;
         // the lanes here are the wave's first ones
         uint32_t through = mine;
-        through += dpp<0x111, 0xF>(through);
-        through += dpp<0x112, 0xF>(through);
-        through += dpp<0x114, 0xF>(through);
-        through += dpp<0x118, 0xF>(through);
-        through += dpp<0x142, 0xA>(through);
-        through += dpp<0x143, 0xC>(through);
+        u64 none = 0;
+        scan_wave(through, none);
         const int last = 63 - __clzll((long long)__ballot(true));
         uint32_t at = 0;
         if ((threadIdx.x & 63u) == 0) at = atomicAdd(&l.listed, (uint32_t)__builtin_amdgcn_readlane((int)through, last));
@@ -483,30 +507,36 @@ __device__ __forceinline__ bool list_firsts(Lds& l, const Measure& m, const Firs
     return true;
 }
 
-// Candidates one a lane of a wave, with what stands before each in their order.
-// Their weights are in units of 2^-FINE, or where they are of one bin in its.
+// Candidates one a lane of the first wave, with what stands before each in their
+// order, which all waves find. Their weights are in units of 2^-FINE, or where
+// they are of one bin in its.
 constexpr int FINE = 56;
 struct Few {
     u64 mine, weight, sum;
     uint32_t n, count;
 
-    __device__ __forceinline__ Few(const u64* from, u64* weights, uint32_t size, const Measure& m, bool one_bin, uint32_t before,
-                                   u64 sum_before)
-        : mine(~0ull), weight(0), sum(sum_before), n(size), count(before) {
+    __device__ __forceinline__ Few(Lds& l, const u64* from, uint32_t size, const Measure& m, bool one_bin,
+                                   uint32_t before, u64 sum_before)
+        : mine(~0ull), weight(0), sum(0), n(size), count(0) {
         const uint32_t lane = threadIdx.x & 63u;
+        if (threadIdx.x < 64u) {
+            if (lane < n) {
+                mine = from[lane];
+                const float x = value_of((uint32_t)(mine >> 32));
+                const uint32_t bin = m.bin(x);
+                weight = scale_down(m.weight(x, bin), one_bin ? 0 : (int)(m.shift + m.power(bin)) - FINE);
+            }
+            l.weights[lane] = weight, l.sums_before[lane] = sum_before, l.counts_before[lane] = before;
+        }
+        __syncthreads();
         if (lane < n) {
-            mine = from[lane];
-            const float x = value_of((uint32_t)(mine >> 32));
-            const uint32_t bin = m.bin(x);
-            weight = scale_down(m.weight(x, bin), one_bin ? 0 : (int)(m.shift + m.power(bin)) - FINE);
+            const u64 of = from[lane];
+            for (uint32_t j = threadIdx.x >> 6; j < n; j += WAVES)
+                if (from[j] < of) count += 1u, sum += l.weights[j];
+            if (count) atomicAdd(&l.counts_before[lane], count), atomicAdd(&l.sums_before[lane], sum);
         }
-        weights[lane] = weight;
-#pragma unroll 4
-        for (uint32_t j = 0; j < n; ++j) {
-            const bool less = from[j] < mine;
-            count += less ? 1u : 0u;
-            sum += less ? weights[j] : 0;
-        }
+        __syncthreads();
+        sum = l.sums_before[lane], count = l.counts_before[lane];
     }
     static __device__ __forceinline__ u64 one(u64 v, uint32_t lane) {
         return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), (int)lane) << 32 |
@@ -531,8 +561,8 @@ __device__ __forceinline__ void find_few(Lds& l, const Measure& m, Target t, uin
     for (uint32_t i = threadIdx.x; i < listed; i += THREADS)
         if (is(l.list[i])) l.few[atomicAdd(&l.picked, 1u)] = l.list[i];
     __syncthreads();
+    const Few few(l, l.few, n, m, true, count, sum);
     if (threadIdx.x < 64u) {
-        const Few few(l.few, l.weights, n, m, true, count, sum);
         u64 through;
         const uint32_t index = few.find(t, through);
         if (threadIdx.x == 0) l.found.index = index, l.found.sum = through;
@@ -702,9 +732,9 @@ struct Counting {
         __syncthreads();
     }
     static __device__ __forceinline__ void add(u64& to, u64 v) {
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
-        if ((threadIdx.x & 63u) == 0) atomicAdd(&to, v);
+        uint32_t none = 0;
+        scan_wave(none, v);
+        if ((threadIdx.x & 63u) == 63u) atomicAdd(&to, v);
     }
 };
 
@@ -774,9 +804,9 @@ __device__ __forceinline__ void choose(const Sample& a, uint32_t r, Lds& l, cons
                 list_values(l, row, value_of(l.keys[1] - 1u), m.top);
             }
             if (l.listed <= FEW) {
+                const Few few(l, l.list, l.listed, m, false, 0, 0);
                 if (threadIdx.x < 64u) {
                     // in units of 2^-FINE
-                    const Few few(l.list, l.weights, l.listed, m, false, 0, 0);
                     u64 through, left = ~0ull;
                     double of = __builtin_ldexp((double)total, FINE - common);
                     if (cut_k) few.find(kth, left), of = (double)left;
@@ -824,6 +854,11 @@ __global__ __launch_bounds__(1024) void k_sample_extent(Sample a) {
 // A row's extent from its chunks' or its waves'.
 __device__ __forceinline__ Extent join_extents(const Extent* parts, uint32_t count) {
     Extent e{-INFINITY, INFINITY, ~0u};
+    if (count <= 16u) {
+        if ((threadIdx.x & 15u) < count) e = parts[threadIdx.x & 15u];
+        e.take_sixteen();
+        return e;
+    }
     for (uint32_t c = threadIdx.x & 63u; c < count; c += 64u) e.take(parts[c]);
     e.take_wave();
     return e;
@@ -942,7 +977,10 @@ int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t tem
     // a chunk for each compute unit, of four values a thread or more
     constexpr uint32_t LEAST = 4u * THREADS, LDS = sizeof(Counting) + sizeof(Lds);
     const uint32_t chunks = std::min((uint32_t)ctx.compute_units / rows, (n + LEAST - 1u) / LEAST);
-    if (chunks <= 1u) {
+    // One launch where a workgroup is through a row before three are (us, one launch
+    // and three: 1 x 16384 18.5 and 21.6, 1 x 32768 24.2 and 22.1; 32 x 32768 25.6
+    // and 27.6, 32 x 50000 32.0 and 29.7; 100 x 50000 33.2 and 36.7)
+    if (chunks <= 1u || n <= 24576u + 512u * rows) {
         TMH_LAUNCH(k_sample_row, dim3(rows), dim3(THREADS), LDS, ctx.stream, a);
     } else {
         a.chunk = (n + chunks - 1u) / chunks;

@@ -202,3 +202,63 @@ def test_lists_of_every_length(dev):
                 ts = np.full(rows, t, np.float32)
                 got = run(dev, x, us, ts, k, ps)
                 assert list(got) == [ref.sample(x[r], u, t, k[r], p) for r in range(rows)]
+
+
+def odd_rows(rng, n):
+    """Rows whose candidates, masks and ties fall in one part of them or across all."""
+    x = rng.normal(0, 2, (14, n)).astype(np.float32)
+    x[0] = -np.sort(-x[0])                      # the first ones next to each other
+    x[1] = np.sort(x[1])
+    x[2, : n - 100] = -np.inf
+    x[3, 7:] = -np.inf
+    x[4] = np.nan
+    x[4, n // 2] = -3.0
+    x[5, rng.permutation(n)[: n // 2]] = np.nan
+    x[6, [5, n // 3, n - 1]] = np.inf
+    x[7] = rng.integers(-2, 3, n)               # ties by the thousand
+    x[8] = 1.25                                 # one value
+    x[9] = np.float32(1.0) + rng.permutation(n).astype(np.float32) * np.float32(2.0 ** -23)
+    x[9, 0], x[9, 1] = -30.0, 1.0 + 2.0 ** -4
+    x[10] = np.finfo(np.float32).min
+    x[10, n - 50:] = 1.0
+    x[11] *= 1e30
+    x[12] = 40.0 - 1e-3 * np.arange(n)          # most of them too far below to count
+    x[13] = -np.inf
+    return x
+
+
+@pytest.mark.parametrize("n", [70003, 131072])
+def test_rows_in_chunks(dev, n):
+    # few long rows, which several workgroups share
+    say("chunks", n)
+    rng = np.random.default_rng(15)
+    x = odd_rows(rng, n)
+    rows = len(x)
+    for trial in range(8):
+        u, t, k, p, m = settings(rng, rows)
+        if trial == 1:
+            k[:], p[:], m[:] = 0, 1.0, 0.0
+        if trial == 2:
+            k[:], p[:], m[:] = 0, 0.95, 0.0
+        if trial == 3:
+            k[:], p[:], m[:] = 3000, 1.0, 0.0
+        if trial == 4:
+            k[:], p[:], m[:] = 40, 0.9, 0.05
+        got = run(dev, x, u, t, k, p, m)
+        assert list(got) == [ref.sample(x[r], u[r], t[r], k[r], p[r], m[r]) for r in range(rows)], trial
+
+
+@pytest.mark.parametrize("n", [500, 70000])
+def test_extreme_temperatures(dev, n):
+    say("temperatures", n)
+    rng = np.random.default_rng(16)
+    t = np.array([1e-38, 1e-30, 1e-10, 1e10, 1e30, 3e38, np.inf, 1e-42], np.float32)
+    rows = t.size
+    x = rng.normal(0, 2, (rows, n)).astype(np.float32)
+    x[:, 11] = x[:, 40] = x[:, n - 2] = 30.0    # three first ones
+    x[4] *= 1e30
+    for u in (0.0, 0.4, 0.99):
+        for k, p in ((0, 1.0), (0, 0.9), (100, 1.0)):
+            us, ks, ps = np.full(rows, u, np.float32), np.full(rows, k, np.int32), np.full(rows, p, np.float32)
+            got = run(dev, x, us, t, ks, ps)
+            assert list(got) == [ref.sample(x[r], us[r], t[r], k, ps[r]) for r in range(rows)], (u, k, p)

@@ -463,12 +463,13 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
  * e^((x - highest) / temperature[r]). The first top_k[r] (int32; below 1: all)
  * stay; of those the shortest run from the front whose weights reach top_p[r]
  * of their sum (1 or more: all); of those the ones of weight at least
- * min_p[r] of the highest; the first always stays. Chosen is the first whose running sum
- * passes u[r] (f32 in [0, 1)) times the sum of what stayed. temperature[r]
- * not above 0 is tmh_argmax. temperature, top_k, top_p and min_p may each be 0
- * (no array): 1, all, 1 and 0. Sums and the weights are in 64 bits: the same
- * inputs give the same ids on every call. Of a sampled row NaN is never chosen
- * while another candidate above -inf is there; n is at most 2^24, rows 65535. */
+ * min_p[r] of the highest; the first always stays. Chosen is the first whose
+ * running sum passes u[r] (f32 in [0, 1)) times the sum of what stayed.
+ * temperature[r] not above 0 is tmh_argmax, one below 1e-38 counts as that.
+ * temperature, top_k, top_p and min_p may each be 0 (no array): 1, all, 1 and 0.
+ * Sums and the weights are in 64 bits: the same inputs give the same ids on
+ * every call. Of a sampled row NaN is never chosen while another candidate
+ * above -inf is there; n is at most 2^24, rows 65535. */
 int tmh_sample(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t temperature, uint64_t top_k,
                uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids);
 

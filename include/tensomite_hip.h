@@ -412,7 +412,8 @@ int tmh_argmax(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t ids
  *
  *   page_table  int32 [sequences, table_width]: sequence s holds position p on
  *               page page_table[s][p / page_size], at place p % page_size;
- *               entries past a sequence's last position are not read
+ *               entries past a sequence's last position are not read, nor are
+ *               those of pages that a window hides from all its new tokens
  *   starts      int32 [sequences + 1]: rows starts[s] ... starts[s+1] - 1 of the
  *               call's tokens are sequence s's new tokens, its newest
  *               positions; rows of no sequence are left as they were
@@ -434,7 +435,7 @@ int tmh_argmax(uint64_t x, uint32_t ldx, uint32_t rows, uint32_t n, uint64_t ids
  * heads, as tmh_rope_write (the same bits in q_dst and an F32 cache; F16 and
  * BF16 elements are the nearest, ties to even), into pages. x rows are `ldx`
  * apart; a position's rotation is its row of the cos/sin tables ([table_rows,
- * width]); a position past them is an index error. */
+ * width]); a position past them is an index error. q_dst may not overlap x. */
 int tmh_rope_write_paged(uint64_t x, uint32_t ldx, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t width,
                          uint64_t cos, uint64_t sin, uint32_t table_rows, uint32_t kind, uint32_t pages,
                          uint32_t page_size, uint64_t page_table, uint32_t table_width, uint32_t sequences,

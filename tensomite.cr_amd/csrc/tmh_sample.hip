@@ -20,7 +20,9 @@
 // Rows of ordinary length go a workgroup each, in one launch. Few long ones go in
 // three, cut in chunks until there is one for each compute unit: chunks' highest
 // and lowest values; their histograms, added to the row's, with each chunk's first
-// candidates; then a workgroup a row. Temperatures count as 1e-38 at least.
+// candidates; then a workgroup a row. Temperatures count as 1e-38 at least. Lists
+// are bounded where they are written, not by what was counted alone: a row that
+// another stream writes meanwhile gives some id, and nothing past an array.
 //
 // Measured: 200 rows of 50257 with cuts 49 us (the first pass 6, at 6.7 TB/s; the
 // histogram 13, its vector operations, about 30 a value; 5 for each list taken from
@@ -505,7 +507,9 @@ __device__ __forceinline__ bool list_firsts(Lds& l, const Measure& m, const Firs
         const First& f = chunks[i / FIRST];
         if (i % FIRST >= f.count) continue;
         const u64 c = f.list[i % FIRST];
-        if (m.bin(value_of((uint32_t)(c >> 32))) <= last) l.list[atomicAdd(&l.listed, 1u)] = c;
+        if (m.bin(value_of((uint32_t)(c >> 32))) > last) continue;
+        const uint32_t at = atomicAdd(&l.listed, 1u);
+        if (at < LIST) l.list[at] = c;
     }
     __syncthreads();
     return true;
@@ -562,10 +566,13 @@ __device__ __forceinline__ void find_few(Lds& l, const Measure& m, Target t, uin
     const uint32_t listed = l.listed;
     if (threadIdx.x == 0) l.picked = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed; i += THREADS)
-        if (is(l.list[i])) l.few[atomicAdd(&l.picked, 1u)] = l.list[i];
+    for (uint32_t i = threadIdx.x; i < listed; i += THREADS) {
+        if (!is(l.list[i])) continue;
+        const uint32_t at = atomicAdd(&l.picked, 1u);
+        if (at < FEW) l.few[at] = l.list[i];
+    }
     __syncthreads();
-    const Few few(l, l.few, n, m, true, count, sum);
+    const Few few(l, l.few, min(n, FEW), m, true, count, sum);
     if (threadIdx.x < 64u) {
         u64 through;
         const uint32_t index = few.find(t, through);
@@ -582,7 +589,7 @@ __device__ __forceinline__ void find_listed(Lds& l, const Measure& m, Target t, 
     const uint32_t listed = l.listed;
     u64 low = (u64)key_low << 32, high = (u64)key_high << 32 | 0xffffffffu, sum = l.found.sum_before;
     uint32_t n = l.found.count, count = l.found.count_before;
-    while (n > FEW) {
+    while (n > FEW && low < high) {
         uint32_t shift = 0;
         while (((high - low) >> shift) >= ZOOM) ++shift;
         __syncthreads();
@@ -914,7 +921,9 @@ __global__ __launch_bounds__(1024) void k_sample_histogram(Sample a) {
     First& first = a.firsts[(size_t)r * a.chunks + chunk];
     const uint32_t before = end;
     part.each<2>([&](float x, uint32_t j) {
-        if (m.within(x) && m.bin(x) < before) first.list[atomicAdd(&listed, 1u)] = (u64)key_of(x) << 32 | j;
+        if (!m.within(x) || m.bin(x) >= before) return;
+        const uint32_t at = atomicAdd(&listed, 1u);
+        if (at < FIRST) first.list[at] = (u64)key_of(x) << 32 | j;
     });
     __syncthreads();
     if (threadIdx.x == 0) first.count = listed, first.end = before;

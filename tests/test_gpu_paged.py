@@ -547,3 +547,33 @@ def test_no_memory_and_no_kernels(dev):
     got = dev.to_array(dst, np.float32, q.size)
     dev.sync()
     assert (got == 0.0).all()
+
+
+@pytest.mark.parametrize("kind", ["F32", "F16", "BF16"])
+@pytest.mark.parametrize("heads,kv,width", [(4, 2, 32), (2, 1, 64), (4, 1, 128), (2, 2, 256)])
+def test_steps_and_chunks_split_in_one_call(dev, kind, heads, kv, width):
+    # row tiles and few rows of one launch, both in parts that one launch joins
+    say("split", kind, heads, kv, width)
+    batch = ref.Batch([(1, 5000), (64, 4100), (0, 12), (3, 2700), (130, 3333)], 32, seed=31, lead=1, trail=2)
+    q, keys, values = inputs(32, batch, heads, kv, width)
+    agree(*attend(dev, kind, batch, q, keys, values), batch)
+    agree(*attend(dev, kind, batch, q, keys, values, window=1500, sinks=70), batch)
+
+
+def test_more_sequences_than_a_wave_has_lanes(dev):
+    say("sequences")
+    rng = np.random.default_rng(33)
+    sizes = [(int(rng.choice([0, 1, 1, 2, 40])), 0) for _ in range(200)]
+    sizes = [(n, n + int(rng.integers(0, 60))) for n, _ in sizes]
+    batch = ref.Batch(sizes, 8, seed=34, lead=3, trail=1)
+    q, keys, values = inputs(35, batch, 4, 2, 64)
+    agree(*attend(dev, "F16", batch, q, keys, values), batch)
+
+
+def test_pages_that_two_sequences_share(dev):
+    # a common prefix: the first four pages of one table are the other's
+    say("shared")
+    batch = ref.Batch([(5, 100), (40, 90)], 16, seed=36)
+    batch.table[1, :4] = batch.table[0, :4]
+    q, keys, values = inputs(37, batch, 4, 2, 64)
+    agree(*attend(dev, "BF16", batch, q, keys, values), batch)

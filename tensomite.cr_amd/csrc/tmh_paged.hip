@@ -958,6 +958,80 @@ __device__ __forceinline__ void attend_tile(const AttendPaged& a, uint32_t block
         load_held(0);
     else
         load_direct(0);
+    // 32 keys from position kg, rows 32 g .. of a stage: whether none of the wave's
+    // rows sees any; their scores; their weights and values
+    const auto hidden = [&](uint32_t kg) { return idle || kg > hi || (kg >= a.sinks && kg + 32u <= window_start(a, lo)); };
+    const auto multiply = [&](const uint8_t* stage, uint32_t g, f32x16& score) {
+        // ahead of other waves' vector operations (512 tokens at the end of 30000,
+        // bf16, 128 wide: 612 us, 596 with it)
+        __builtin_amdgcn_s_setprio(1);
+        score = f32x16{} * 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < W / 16u; ++k) {
+            Operand<CP> o;
+            const uint32_t row = g * 32u + col;
+#pragma unroll
+            for (uint32_t p = 0; p < CP; ++p)
+                o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
+            score = multiply_parts32<KIND>(o, query[k], score);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    const auto weigh = [&](const uint8_t* stage, uint32_t g, uint32_t kg, f32x16& score) {
+        const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
+        if (!whole) {
+#pragma unroll
+            for (uint32_t j = 0; j < 16u; ++j)
+                if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
+        }
+        float best = score[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
+        if (__any(best > limit)) {
+            best = fmaxf(best, __shfl_xor(best, 32, 64));
+            if (best > limit) {
+                const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((zero - best) * undo + HEADROOM);
+                zero = best - HEADROOM * power;
+                limit = best + SLACK * power;
+                total *= keep;
+#pragma unroll
+                for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
+            }
+        }
+        score -= zero;
+        if (KIND == TMH_CACHE_F16 && scaled) {
+            asm volatile("");  // a branch: most rows have no power
+#pragma unroll
+            for (int j = 0; j < 16; ++j) score[j] *= undo;
+        }
+        Operand<NP> weight[2];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
+            sum += e0;
+            sum += e1;
+            split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
+        }
+        total += sum;
+#pragma unroll
+        for (uint32_t d = 0; d < W / 32u; ++d)
+#pragma unroll
+            for (uint32_t c = 0; c < 2u; ++c) {
+                // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
+                Operand<CP> o;
+                const uint32_t row = g * 32u + c * 16u + half * 4u + col % 16u / 4u;
+                const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
+#pragma unroll
+                for (uint32_t p = 0; p < CP; ++p) {
+                    const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
+                    const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
+                    const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
+                    o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
+                }
+                out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
+            }
+    };
     for (uint32_t i = 0; i < steps; ++i) {
         const uint8_t* stage = lds;
         if constexpr (T::F32) {
@@ -975,79 +1049,13 @@ __device__ __forceinline__ void attend_tile(const AttendPaged& a, uint32_t block
         const bool looks = i + 2u < steps && wave == (i & 3u);
         uint32_t ahead = 0;
         if (looks) ahead = w.cache_row_for(a, first_key(i + 2u) + lane % KT);
-        const uint32_t k0 = first_key(i);
 #pragma unroll
         for (uint32_t g0 = 0; g0 < KT / 32u; g0 += SHARES) {
-            const uint32_t g = g0 + keys_of, kg = k0 + g * 32u;
-            // keys that none of the wave's rows sees
-            if (idle || kg > hi || (kg >= a.sinks && kg + 32u <= window_start(a, lo))) continue;
-            // ahead of other waves' vector operations (512 tokens at the end of 30000,
-            // bf16, 128 wide: 612 us, 596 with it)
-            __builtin_amdgcn_s_setprio(1);
-            f32x16 score = f32x16{} * 0.0f;
-#pragma unroll
-            for (uint32_t k = 0; k < W / 16u; ++k) {
-                Operand<CP> o;
-                const uint32_t row = g * 32u + col;
-#pragma unroll
-                for (uint32_t p = 0; p < CP; ++p)
-                    o.part[p] = *(const u32x4*)(stage + p * T::PART + row * W * 2u + T::swizzle(k * 2u + half, row) * 16u);
-                score = multiply_parts32<KIND>(o, query[k], score);
-            }
-            __builtin_amdgcn_s_setprio(0);
-            const bool whole = kg + 31u <= lo && (a.window == 0u || hi - kg < a.window || kg + 31u < a.sinks);
-            if (!whole) {
-#pragma unroll
-                for (uint32_t j = 0; j < 16u; ++j)
-                    if (!sees(a, pos, kg + j / 4u * 8u + half * 4u + j % 4u)) score[j] = -INFINITY;
-            }
-            float best = score[0];
-#pragma unroll
-            for (int j = 1; j < 16; ++j) best = fmaxf(best, score[j]);
-            if (__any(best > limit)) {
-                best = fmaxf(best, __shfl_xor(best, 32, 64));
-                if (best > limit) {
-                    const float keep = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((zero - best) * undo + HEADROOM);
-                    zero = best - HEADROOM * power;
-                    limit = best + SLACK * power;
-                    total *= keep;
-#pragma unroll
-                    for (uint32_t d = 0; d < W / 32u; ++d) out[d] *= keep;
-                }
-            }
-            score -= zero;
-            if (KIND == TMH_CACHE_F16 && scaled) {
-                asm volatile("");  // a branch: most rows have no power
-#pragma unroll
-                for (int j = 0; j < 16; ++j) score[j] *= undo;
-            }
-            Operand<NP> weight[2];
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(score[j]), e1 = __builtin_amdgcn_exp2f(score[j + 1]);
-                sum += e0;
-                sum += e1;
-                split_pair<KIND>(weight[j / 8], j % 8 / 2, e0, e1);
-            }
-            total += sum;
-#pragma unroll
-            for (uint32_t d = 0; d < W / 32u; ++d)
-#pragma unroll
-                for (uint32_t c = 0; c < 2u; ++c) {
-                    // keys 16c + 4 half .. + 3 and 8 further; 16 columns a lane group
-                    Operand<CP> o;
-                    const uint32_t row = g * 32u + c * 16u + half * 4u + col % 16u / 4u;
-                    const uint32_t chunk = d * 4u + col / 16u * 2u + col % 4u / 2u;
-#pragma unroll
-                    for (uint32_t p = 0; p < CP; ++p) {
-                        const uint8_t* from = stage + (CP + p) * T::PART + col % 2u * 8u;
-                        const uint64_t early = read_turned(from + row * W * 2u + T::swizzle(chunk, row) * 16u);
-                        const uint64_t late = read_turned(from + (row + 8u) * W * 2u + T::swizzle(chunk, row + 8u) * 16u);
-                        o.part[p] = u32x4{(uint32_t)early, (uint32_t)(early >> 32), (uint32_t)late, (uint32_t)(late >> 32)};
-                    }
-                    out[d] = multiply_parts32<KIND>(o, weight[c], out[d]);
-                }
+            const uint32_t g = g0 + keys_of, kg = first_key(i) + g * 32u;
+            if (hidden(kg)) continue;
+            f32x16 score;
+            multiply(stage, g, score);
+            weigh(stage, g, kg, score);
         }
         if (looks && lane < KT) cache_rows[i & 1u][lane] = ahead;
     }
@@ -1114,9 +1122,11 @@ __device__ __forceinline__ void attend_tile(const AttendPaged& a, uint32_t block
     if (any) plain_rows<KIND>(a, w, part, redo);
 }
 
-// One sequence, of more rows than few.
+// One sequence, of more rows than few. Registers for three waves a SIMD where LDS
+// has room for as many (1024 tokens after 3000, 9 heads of 64, bf16: 61 us with two
+// waves, 53 with three; the batch below, whose workgroups are shorter, loses by it).
 template <uint32_t KIND, uint32_t W>
-__global__ __launch_bounds__(256) void k_attend_tile(AttendPaged a) {
+__global__ __launch_bounds__(256, W <= 64u && KIND != TMH_CACHE_F32 ? 3 : 1) void k_attend_tile(AttendPaged a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     attend_tile<KIND, W>(a, blockIdx.x, lds);
 }

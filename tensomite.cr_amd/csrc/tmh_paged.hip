@@ -1372,11 +1372,16 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
                    few_groups > (uint32_t)ctx.compute_units ? 32u : 8u);
     }
     if (has_more) {
-        // row tiles of all sequences, at most; two workgroups a compute unit
+        // Row tiles of all sequences, at most. Two workgroups a compute unit, or four
+        // of those with 64 rows that have the most to do besides products, f32 ones,
+        // or the least, 32 columns (1024 tokens after 3000, 9 heads of 64, f32 99 us with
+        // two and 80 with four, f16 47.5 and 51.6; two of 1000 after 4000, 4 heads of
+        // 32, f16 36.7 and 32.8)
         const uint64_t all = (uint64_t)tokens * group;
         more_groups = (all / more.row_tile + std::min<uint64_t>(sequences, all / (FEW_ROWS + 1u))) * kv_heads;
         if (more.alone) more_groups = (all + more.row_tile - 1u) / more.row_tile * kv_heads;
-        set_shares(more, more_groups, most_tiles(a, more.row_tile), 2u * ctx.compute_units, 8u);
+        const uint32_t each = width <= 32u || (width <= 64u && kind == TMH_CACHE_F32) ? 4u : 2u;
+        set_shares(more, more_groups, most_tiles(a, more.row_tile), each * ctx.compute_units, 8u);
     }
     if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / 8u)
         return TMH_ERROR_SHAPE;

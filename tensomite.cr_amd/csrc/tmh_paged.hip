@@ -1272,11 +1272,10 @@ uint64_t most_tiles(const AttendPaged& a, uint32_t tokens) {
     return std::min<uint64_t>(all, ((uint64_t)a.sinks + KEYS - 1u) / KEYS + ((uint64_t)a.window + tokens + KEYS) / KEYS + 1u);
 }
 
-// Shares of the keys for `groups` row tiles of at most `tiles` tiles of keys:
-// so that there are at most `wanted` workgroups, or one a row tile, of at least
+// Shares of at most `tiles` tiles of keys: no more than `parts`, of at least
 // `least` tiles each.
-void set_shares(AttendPaged& a, uint64_t groups, uint64_t tiles, uint64_t wanted, uint32_t least) {
-    a.share = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(least, (groups * tiles + wanted - 1u) / wanted), 0x7fffffffu);
+void set_shares(AttendPaged& a, uint64_t tiles, uint64_t parts, uint32_t least) {
+    a.share = (uint32_t)std::max<uint64_t>(least, (tiles + parts - 1u) / parts);
     a.splits = (uint32_t)std::max<uint64_t>(1u, (tiles + a.share - 1u) / a.share);
 }
 
@@ -1363,13 +1362,21 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
     l.row_tiles = (few.room + FEW_TILE - 1u) / FEW_TILE;
     uint64_t few_groups = 0, more_groups = 0;
     if (!more.alone) {
-        // four workgroups a compute unit, a share of at least eight tiles of keys
-        // (two steps a wave; a join costs more than that: 512 positions 9.0 us in
-        // two launches, 7.5 in one), or thirty-two where row tiles alone are more
-        // than compute units (48 windows of 1024: shares of 8 tiles 97 us, whole 84)
+        // As many workgroups as run at once by their registers, no more: four a
+        // compute unit up to 64 columns, two to 128, one above (4 sequences of up to
+        // 131072, 8 kv heads of 128, f16: 275 us with two a compute unit, 290 with
+        // four; 4 of 4000, 5 of 256: 24 with one, 33 with more). A share's time goes
+        // with its tiles, the join's with the parts, their sum is least at a root
+        // (20000 positions, 8 kv heads of 128, f16, 313 tiles: 27.4 us in 16 parts, 23.6
+        // in 32, 27.1 in 63). Shares are four tiles at least, one step a wave, and
+        // eight are one share: a second launch costs more than it gains (512
+        // positions, 3 kv heads of 64: 7.9 us in one launch, 10.1 in two; 2000: 11.9 with
+        // shares of eight tiles, 10.2 of four).
         few_groups = (uint64_t)sequences * kv_heads * l.row_tiles;
-        set_shares(few, few_groups, most_tiles(a, FEW_ROWS), 4u * ctx.compute_units,
-                   few_groups > (uint32_t)ctx.compute_units ? 32u : 8u);
+        const uint64_t at_once = (width <= 64u ? 4u : width <= 128u ? 2u : 1u) * (uint64_t)ctx.compute_units;
+        const uint64_t tiles = most_tiles(a, FEW_ROWS);
+        const uint64_t parts = std::min(at_once / few_groups, (uint64_t)(2.0 * std::sqrt((double)tiles)));
+        set_shares(few, tiles, std::max<uint64_t>(parts, 1u), tiles <= 8u ? 8u : 4u);
     }
     if (has_more) {
         // Row tiles of all sequences, at most. Two workgroups a compute unit, or four
@@ -1380,8 +1387,8 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
         const uint64_t all = (uint64_t)tokens * group;
         more_groups = (all / more.row_tile + std::min<uint64_t>(sequences, all / (FEW_ROWS + 1u))) * kv_heads;
         if (more.alone) more_groups = (all + more.row_tile - 1u) / more.row_tile * kv_heads;
-        const uint32_t each = width <= 32u || (width <= 64u && kind == TMH_CACHE_F32) ? 4u : 2u;
-        set_shares(more, more_groups, most_tiles(a, more.row_tile), each * ctx.compute_units, 8u);
+        const uint64_t wanted = (width <= 32u || (width <= 64u && kind == TMH_CACHE_F32) ? 4u : 2u) * (uint64_t)ctx.compute_units;
+        if (more_groups) set_shares(more, most_tiles(a, more.row_tile), (wanted + more_groups - 1u) / more_groups, 8u);
     }
     if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / 8u)
         return TMH_ERROR_SHAPE;

@@ -577,3 +577,20 @@ def test_pages_that_two_sequences_share(dev):
     batch.table[1, :4] = batch.table[0, :4]
     q, keys, values = inputs(37, batch, 4, 2, 64)
     agree(*attend(dev, "BF16", batch, q, keys, values), batch)
+
+
+@pytest.mark.parametrize("max_new,max_length", [(500, 4000), (500, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1)])
+@pytest.mark.parametrize("sizes", [[(1, 20), (2, 133)], [(9, 9)], [(60, 300), (1, 1000)]])
+def test_loose_bounds(dev, max_new, max_length, sizes):
+    # announced: more new tokens and longer sequences than there are
+    say("loose", max_new, max_length, sizes)
+    batch = ref.Batch(sizes, 16, seed=38, lead=1)
+    q, keys, values = inputs(39, batch, 4, 2, 64)
+    cache, k, v = cache_of(dev, "F16", batch, 2, keys, values)
+    b = batch.on(dev)
+    b.max_new, b.max_length = max_new, max_length
+    dst = dev.from_array(np.full(q.shape, 7.25, np.float32))
+    dev.attention_paged(dev.from_array(q), batch.tokens, 4, cache, b, 0.125, dst=dst)
+    got = dev.to_array(dst, np.float32, q.size).reshape(q.shape)
+    dev.sync()
+    agree(got, *ref.attention(q, k, v, batch, 0.125), batch)

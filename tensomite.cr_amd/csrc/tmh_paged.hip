@@ -1203,22 +1203,23 @@ __device__ __forceinline__ void join_row(const AttendPaged& a, const Rows& w, ui
     }
 }
 
-// Joins the rows that came in parts: a quarter of a row tile, a quarter of that a
-// wave, in the first 4 `groups` workgroups; then few rows, a wave a row, by
+// Joins the rows that came in parts: a sixteenth of a row tile, a quarter of that a
+// wave, in the first JOINS `groups` workgroups; then few rows, a wave a row, by
 // sequence, kv head and row, `count` of them.
+constexpr uint32_t JOINS = 16;
 __global__ __launch_bounds__(256) void k_attend_join(AttendPaged more, AttendPaged few, uint32_t groups, uint32_t count) {
     __shared__ f32x4 lanes[4][64];
     const uint32_t wave = wave_index();
     Rows w;
-    if (blockIdx.x < 4u * groups) {
-        const uint32_t b = blockIdx.x / 4u, quarter = blockIdx.x % 4u;
+    if (blockIdx.x < JOINS * groups) {
+        const uint32_t b = blockIdx.x / JOINS, rows = more.row_tile / (4u * JOINS);
         w.kh = b % more.p.kv_heads;
         if (!find_row_tile(more, b / more.p.kv_heads, 0, w) || w.parts == 1u) return;
-        const uint32_t from = quarter * (more.row_tile / 4u) + wave * (more.row_tile / 16u);
-        for (uint32_t i = from; i < min(from + more.row_tile / 16u, w.count); ++i) join_row(more, w, w.first + i, lanes[wave]);
+        const uint32_t from = (blockIdx.x % JOINS * 4u + wave) * rows;
+        for (uint32_t i = from; i < min(from + rows, w.count); ++i) join_row(more, w, w.first + i, lanes[wave]);
         return;
     }
-    uint32_t b = (blockIdx.x - 4u * groups) * 4u + wave;
+    uint32_t b = (blockIdx.x - JOINS * groups) * 4u + wave;
     if (b >= count) return;
     const uint32_t r = b % few.room;
     b /= few.room;
@@ -1390,7 +1391,7 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
         const uint64_t wanted = (width <= 32u || (width <= 64u && kind == TMH_CACHE_F32) ? 4u : 2u) * (uint64_t)ctx.compute_units;
         if (more_groups) set_shares(more, most_tiles(a, more.row_tile), (wanted + more_groups - 1u) / more_groups, 8u);
     }
-    if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / 8u)
+    if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / (2u * JOINS))
         return TMH_ERROR_SHAPE;
     l.few_groups = (uint32_t)few_groups, l.more_groups = (uint32_t)more_groups;
     const size_t few_parts = few.splits > 1u ? (size_t)sequences * kv_heads * few.room * few.splits : 0;
@@ -1411,7 +1412,7 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
     hipError_t e = hipGetLastError();
     const uint32_t groups = more_parts ? l.more_groups : 0u, count = few_parts ? sequences * kv_heads * few.room : 0u;
     if (e == hipSuccess && (groups || count)) {
-        TMH_LAUNCH(k_attend_join, dim3(4u * groups + (count + 3u) / 4u), dim3(256), 0, ctx.stream, more, few, groups, count);
+        TMH_LAUNCH(k_attend_join, dim3(JOINS * groups + (count + 3u) / 4u), dim3(256), 0, ctx.stream, more, few, groups, count);
         e = hipGetLastError();
     }
     if (e == hipSuccess) note_launch(ctx.index, 1, true);

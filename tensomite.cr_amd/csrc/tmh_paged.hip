@@ -1380,16 +1380,36 @@ int tmh_attention_paged(uint64_t q, uint32_t ldq, uint32_t tokens, uint32_t head
         set_shares(few, tiles, std::max<uint64_t>(parts, 1u), tiles <= 8u ? 8u : 4u);
     }
     if (has_more) {
-        // Row tiles of all sequences, at most. Two workgroups a compute unit, or four
-        // of those with 64 rows that have the most to do besides products, f32 ones,
-        // or the least, 32 columns (1024 tokens after 3000, 9 heads of 64, f32 99 us with
-        // two and 80 with four, f16 47.5 and 51.6; two of 1000 after 4000, 4 heads of
-        // 32, f16 36.7 and 32.8)
-        const uint64_t all = (uint64_t)tokens * group;
-        more_groups = (all / more.row_tile + std::min<uint64_t>(sequences, all / (FEW_ROWS + 1u))) * kv_heads;
-        if (more.alone) more_groups = (all + more.row_tile - 1u) / more.row_tile * kv_heads;
-        const uint64_t wanted = (width <= 32u || (width <= 64u && kind == TMH_CACHE_F32) ? 4u : 2u) * (uint64_t)ctx.compute_units;
-        if (more_groups) set_shares(more, most_tiles(a, more.row_tile), (wanted + more_groups - 1u) / more_groups, 8u);
+        // Row tiles of all sequences, at most; and about, a sequence's last half full.
+        const uint64_t all = (uint64_t)tokens * group, ends = std::min<uint64_t>(sequences, all / (FEW_ROWS + 1u));
+        more_groups = (all / more.row_tile + ends) * kv_heads;
+        uint64_t about = (all / more.row_tile + (ends + 1u) / 2u) * kv_heads;
+        if (more.alone) about = more_groups = (all + more.row_tile - 1u) / more.row_tile * kv_heads;
+        // Again as many as run at once (beside few rows two a compute unit at most),
+        // and no second round of a few (1024 tokens after 3000, 9 heads of 64, 144 row
+        // tiles: f16 48.0 us in 4 parts, 43.1 in 5, 52.2 in 6; f32 95.9 in 2, 75.0 in 3,
+        // 99.4 in 4). Row tiles see from 1 - f of the tiles to all: of p parts they
+        // have p (1 - f / 2) + 1 / 2 on average, p where that is less than one apart.
+        // Prompts, f near 1, are even enough in three (1500 tokens, 16 heads of 128, f16:
+        // 60.5 us whole, 53.0, 49.9, 59.5 in 2, 3, 4), and where one round would leave
+        // them whole their last tiles would run on alone, so that two are taken if row
+        // tiles are few or long (4096 tokens, 8 heads of 256, f16: 335 us whole, 252 in
+        // 3; but 1500 tokens, 32 heads of 64, 38 whole, 73 in 3). Shares as above; eight
+        // tiles are one: a prompt of 512, f16, 15.2 us in one launch, 16.6 in two.
+        const bool f32 = kind == TMH_CACHE_F32, narrow = width <= 32u || (width <= 64u && !f32);
+        const uint64_t each = narrow ? (more.alone ? 3u : 2u) : width <= 64u || (width <= 128u && !f32) ? 2u : 1u;
+        const uint64_t at_once = each * ctx.compute_units, tiles = most_tiles(a, more.row_tile);
+        const double f = std::min(1.0, (double)max_new / std::max(1.0, (double)max_length));
+        const auto parts_for = [&](uint64_t groups) {
+            const double p = (double)groups / (double)std::max<uint64_t>(about, 1u);
+            return f * p < 1.0 ? p : (p - 0.5) / (1.0 - f / 2.0);
+        };
+        double parts = parts_for(at_once);
+        if (f > 0.9) {
+            if (parts < 2.0 && (4u * about <= 3u * at_once || (about <= at_once && tiles >= 48u))) parts = parts_for(2u * at_once);
+            parts = std::min(parts, 3.0);
+        }
+        set_shares(more, tiles, (uint64_t)std::max(parts, 1.0), tiles <= 8u ? 8u : 4u);
     }
     if (few_groups * few.splits + more_groups * more.splits > MOST_GROUPS || more_groups > MOST_GROUPS / (2u * JOINS))
         return TMH_ERROR_SHAPE;

@@ -493,7 +493,7 @@ __device__ __forceinline__ float power_for(float largest) {
 // transposed, keys down and queries across: a lane then holds weights of one
 // query and of eight keys, which is what the second product wants of it, with
 // the keys in the order 4g..4g+3, 16+4g..16+4g+3 for lane group g.
-// Measured: 376832 positions of 8 kv heads of 128, f16, 285 us, 5.4 TB/s; 48
+// Measured: 376832 positions of 8 kv heads of 128, f16, 270 us, 5.7 TB/s; 48
 // windows of 1024, f32, 84 us, 4.8 TB/s; 8 sequences of 2048 and less with 32 kv
 // heads of 64, bf16, 19 us, 4.7 TB/s; 512 positions of 3 kv heads 7.5 us, all of it
 // latency (a page looked up, keys read, the waves' sums joined).
@@ -783,9 +783,9 @@ __device__ __forceinline__ f32x16 multiply_parts32(const Operand<Split<KIND>::CA
 // of the wave, which are the keys its second operand is given. F16 and BF16 tiles
 // come by direct loads into one of two buffers while the other is used; F32 ones are
 // split in parts on the way through registers, once for the four waves.
-// Measured: 512 tokens after 30000, 32 heads of 128 over 8, bf16: 577 us, 433
+// Measured: 512 tokens at the end of 30000, 32 heads of 128 over 8, bf16: 575 us, 434
 // TFLOP/s of attention and three times that of products; a prompt of 2048, 32 heads
-// of 64, f16: 51.5 us, 334 TFLOP/s and twice that.
+// of 64, f16: 52 us, 330 TFLOP/s and twice that.
 // Rows up to 64 columns wide go 64 a workgroup, whose waves have half of the keys
 // of a step each (2048-token prompt, 32 heads of 64, f16: 53 us; 128 rows: 72).
 template <uint32_t KIND, uint32_t W>
@@ -1134,7 +1134,7 @@ __global__ __launch_bounds__(256, W <= 64u && KIND != TMH_CACHE_F32 ? 3 : 1) voi
 // A batch with sequences of both kinds: row tiles in the first `tiles`
 // workgroups, few rows behind them, so that each fills what the other leaves
 // (chunks and decode steps of 12 sequences, f32, 9 heads of 64: two launches in
-// turn 36.5 us, 25.1 so).
+// turn 36.5 us, 24.4 so).
 template <uint32_t KIND, uint32_t W>
 __global__ __launch_bounds__(256) void k_attend_mixed(AttendPaged more, AttendPaged few, uint32_t tiles, uint32_t row_tiles) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -1147,7 +1147,7 @@ __global__ __launch_bounds__(256) void k_attend_mixed(AttendPaged more, AttendPa
 // Joins the parts of row r, by a wave: each part brought to the highest reference
 // and added. The parts wait in L2 or memory, so latency bounds it: a load takes
 // 64 / (width / 4) parts, and eight loads go out before the first is used (256 rows
-// of up to 4 parts 4 us, 16384 of 4 parts of 128 columns 18).
+// of up to 4 parts 4 us, 16384 of 4 parts of 128 columns 14).
 __device__ __forceinline__ void join_row(const AttendPaged& a, const Rows& w, uint32_t r, f32x4* lanes) {
     const uint32_t lane = threadIdx.x & 63u, width = a.p.width, quads = width / 4u;
     const size_t at = w.place(a, r);
